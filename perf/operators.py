@@ -7,8 +7,8 @@ With ``own`` false ``run`` computes them from elementary tensor operations; with
 * select: logits [groups * beams, vocab] (32-bit) and the beams' summed log-probabilities; the ``keep`` best (beam, token) pairs of every
   group by summed log-probability, the lowest beam * vocab + token first among equals.  A place without a beam has a score of -inf, a
   forbidden token a logit of -inf; candidates that do not exist are (-inf, -1, -1).
-* reorder: tensors [pool, ...] of which every beam holds one row (a page of keys and values, a recurrent state): the row of beam b becomes
-  what the row of its parent was.
+* reorder: tensors [pool, ...] (or [layers, pool, ...]) of which every beam holds one row (a page of keys and values, a recurrent state):
+  the row of beam b becomes what the row of its parent was.
 * attention: softmax(scale q K^T) V for one query row a beam.  A page of the cache holds, head by head, its keys row by row and its values
   dimension by dimension.  Rows that nobody has written are no numbers.
 """
@@ -27,9 +27,9 @@ def listed():
         return {"name": name, "op": "select", "groups": groups, "beams": beams, "vocab": vocab, "keep": keep, "live": live or beams,
                 "banned": banned}
 
-    def reorder(name, layers, row, pool, groups, beams, moved, dtype="bfloat16", row2=0):
+    def reorder(name, layers, row, pool, groups, beams, moved, dtype="bfloat16", row2=0, stacked=True):
         return {"name": name, "op": "reorder", "layers": layers, "row": row, "row2": row2, "pool": pool, "groups": groups, "beams": beams,
-                "moved": moved, "dtype": dtype}
+                "moved": moved, "dtype": dtype, "stacked": stacked}
 
     def attention(name, groups, beams, heads, kv_heads, dim, length, behind, page=16, dtype="bfloat16"):
         return {"name": name, "op": "attention", "groups": groups, "beams": beams, "heads": heads, "kv_heads": kv_heads, "dim": dim,
@@ -49,7 +49,7 @@ def listed():
         # the same for eight requests of eight beams on 48 layers of 25 heads
         reorder("reorder-pages-1.5b-8x8", 48, 2 * 25 * 16 * 64, 160, 8, 8, 4),
         # recurrent layers: a short filter's inputs and a 32-bit matrix a head
-        reorder("reorder-states-4x8", 16, 16 * 128 * 128, 32, 4, 8, 5, dtype="float32", row2=3 * 1025),
+        reorder("reorder-states-4x8", 16, 16 * 128 * 128, 32, 4, 8, 5, dtype="float32", row2=3 * 1025, stacked=False),
         # one request of four beams behind a prompt of 512 tokens
         attention("attention-1x4-512", 1, 4, 12, 12, 64, 531, 19),
         # eight requests of eight beams at GPT-2's longest contexts
@@ -74,9 +74,8 @@ def draw(rng):
     if op == "reorder":
         layers, groups, beams = log(1, 60), log(1, 12), log(2, 16)
         dtype = rng.choice(("bfloat16", "float32"))
-        row = min(log(500, 300000), 600_000_000 // (layers * groups * beams * 4)) // 2 * 2
-        return {"op": op, "layers": layers, "row": row, "row2": rng.choice((0, 0, 2 * rng.randint(1, 3000))),
-                "pool": groups * beams + rng.randint(0, 20), "groups": groups, "beams": beams, "moved": rng.randint(1, beams - 1), "dtype": dtype}
+        row, stacked = min(log(500, 300000), 600_000_000 // (layers * groups * beams * 4)) // 2 * 2, rng.random() < 0.6
+        return {"op": op, "layers": layers, "row": row, "row2": 0 if stacked else rng.choice((0, rng.randint(1, 6000))), "stacked": stacked, "pool": groups * beams + rng.randint(0, 20), "groups": groups, "beams": beams, "moved": rng.randint(1, beams - 1), "dtype": dtype}
     groups, beams, kv_heads = log(1, 16), log(2, 16), log(1, 25)
     heads = kv_heads * rng.choice((1, 1, 2, 4, 5))
     dim, dtype = rng.choice((32, 48, 64, 64, 80, 128)), rng.choice(("bfloat16", "bfloat16", "float32"))
@@ -123,7 +122,10 @@ def prepare(case, seed):
                  "scratch": torch.empty(1 << 22, device=DEV)}
     elif case["op"] == "reorder":
         dtype, pool = TYPES[case["dtype"]], case["pool"]
-        tensors = [torch.randn(pool, case["row"], device=DEV, generator=g).to(dtype) for _ in range(case["layers"])]
+        if case["stacked"]:
+            tensors = [torch.randn(case["layers"], pool, case["row"], device=DEV, generator=g).to(dtype)]
+        else:
+            tensors = [torch.randn(pool, case["row"], device=DEV, generator=g).to(dtype) for _ in range(case["layers"])]
         if case["row2"]:
             tensors += [torch.randn(pool, case["row2"], device=DEV, generator=g) for _ in range(case["layers"])]
         slots = torch.randperm(pool, generator=h)[:G * B].view(G, B).to(torch.int32)
@@ -187,7 +189,8 @@ def _select(state):
 def _reorder(state):
     from_rows = torch.gather(state["slots"].long(), 1, state["parents"].long()).view(-1)
     to_rows = state["slots"].long().view(-1)
-    return [t.index_copy_(0, to_rows, t[from_rows]) for t in state["tensors"]]
+    dim = 1 if state["case"]["stacked"] else 0
+    return [t.index_copy_(dim, to_rows, t.index_select(dim, from_rows)) for t in state["tensors"]]
 
 
 def _attention(state):
@@ -213,7 +216,7 @@ def run(state):
             scores, parents, tokens = ops.beam_select(state["logits"], state["scores"], case["beams"], *state["out"], workspace=state["scratch"])
             return {"scores": scores, "parents": parents, "tokens": tokens}
         if case["op"] == "reorder":
-            return ops.state_reorder(state["tensors"], state["slots"], state["parents"])
+            return ops.state_reorder(state["tensors"], state["slots"], state["parents"], dim=1 if case["stacked"] else 0)
         splits = ops.beam_splits(case["groups"], case["beams"], case["heads"], case["kv_heads"], case["dim"], state["table"].shape[1], case["page"])
         return ops.attention_beams(state["q"], state["cache"], state["table"], state["lens"], state["shared"], case["beams"], case["heads"],
                                    case["dim"] ** -0.5, None, state["out"], splits, state["scratch"])
@@ -244,8 +247,9 @@ def exact(case, seed):
         out = []
         for t in state["tensors"]:
             before = t.double()
+            rows = before.transpose(0, 1) if case["stacked"] else before
             for to, came in moves:                        # (who is continued stays where it was)
-                before[to] = before[came]
+                rows[to] = rows[came]
             out.append(before)
         return out
     S, Hq, Hkv, D, page = case["groups"] * case["beams"], case["heads"], case["kv_heads"], case["dim"], case["page"]
