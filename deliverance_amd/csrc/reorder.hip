@@ -1,0 +1,83 @@
+// Rows of many tensors reordered in place: of every group of B places, the row of place b becomes what the row of place
+// parent[b] was, in every tensor.  (What the beams of a search keep, pages of keys and values that are being written and
+// recurrent states, follows the beams that were chosen.)
+//
+// A thread holds one column of a row for all places of a group: it reads the columns of the rows that move, all of them, and only
+// then writes.  No other thread touches its columns, so parents may be any permutation, with repeats, and no copy is made.
+// Rows that stay are neither read nor written.
+#include "common.h"
+
+#define REORDER_TENSORS 96       // of a launch (the table is a kernel argument: nothing is uploaded, a recorded launch keeps it)
+#define REORDER_MAX 64           // places of a group
+#define REORDER_THREADS 256
+
+struct ReorderTable {
+  void* data[REORDER_TENSORS];
+  int units[REORDER_TENSORS];    // of a row: 16 bytes each (WIDE) or 4
+};
+
+// NB: places that a thread has registers for
+template <typename U, int NB>
+__global__ void __launch_bounds__(REORDER_THREADS)
+reorder_kernel(const ReorderTable table, const int* __restrict__ slots, const int* __restrict__ parents, int B, int pool) {
+  const int units = table.units[blockIdx.y], c = blockIdx.x * REORDER_THREADS + threadIdx.x;
+  if (c >= units) return;
+  U* data = (U*)table.data[blockIdx.y];
+  const int* slot = slots + (size_t)blockIdx.z * B;
+  const int* parent = parents + (size_t)blockIdx.z * B;
+  U v[NB];
+  int to[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    to[b] = -1;
+    if (b >= B) continue;
+    const int p = parent[b], s = slot[b];
+    if (p == b || (unsigned)p >= (unsigned)B || (unsigned)s >= (unsigned)pool) continue;
+    const int from = slot[p];
+    if ((unsigned)from >= (unsigned)pool || from == s) continue;
+    v[b] = data[(size_t)from * units + c];
+    to[b] = s;
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (to[b] >= 0) data[(size_t)to[b] * units + c] = v[b];
+}
+
+// n tensors [layers, pool, row]; `data`, `row_bytes` (whole 4-byte words) and `layers` are host arrays.
+extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const int* layers, int n, int pool, const int* slots,
+                                const int* parents, int G, int B, void* stream) {
+  DA_REQUIRE(n >= 0 && G >= 0 && G <= 65535 && B > 0 && B <= REORDER_MAX && pool >= 0,
+             "state_reorder: bad sizes (tensors=%d rows=%d groups=%d places=%d; at most %d places)", n, pool, G, B, REORDER_MAX);
+  for (int i = 0; i < n; ++i)
+    DA_REQUIRE(row_bytes[i] > 0 && row_bytes[i] % 4 == 0 && row_bytes[i] < (1L << 32) && (uintptr_t)data[i] % 4 == 0 && layers[i] >= 0,
+               "state_reorder: %d layers with a row of %ld bytes: not whole words, or too long", layers[i], row_bytes[i]);
+  if (n == 0 || G == 0 || B == 1 || pool == 0) return 0;
+  auto is_wide = [&](int i) { return B <= 16 && row_bytes[i] % 16 == 0 && (uintptr_t)data[i] % 16 == 0; };
+  for (int wide = 0; wide < 2; ++wide) {
+    ReorderTable table;
+    int count = 0, longest = 0;
+    auto launch = [&]() {
+      if (!count) return;
+      const dim3 grid(da_ceil_div(longest, REORDER_THREADS), count, G), block(REORDER_THREADS);
+      hipStream_t s = (hipStream_t)stream;
+      if (wide && B <= 4) hipLaunchKernelGGL((reorder_kernel<uint4, 4>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (wide && B <= 8) hipLaunchKernelGGL((reorder_kernel<uint4, 8>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (wide) hipLaunchKernelGGL((reorder_kernel<uint4, 16>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (B <= 16) hipLaunchKernelGGL((reorder_kernel<uint32_t, 16>), grid, block, 0, s, table, slots, parents, B, pool);
+      else hipLaunchKernelGGL((reorder_kernel<uint32_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
+      count = longest = 0;
+    };
+    for (int i = 0; i < n; ++i) {
+      if ((int)is_wide(i) != wide) continue;
+      for (int layer = 0; layer < layers[i]; ++layer) {
+        table.data[count] = (char*)data[i] + (long)layer * pool * row_bytes[i];
+        table.units[count] = (int)(row_bytes[i] / (wide ? 16 : 4));
+        longest = table.units[count] > longest ? table.units[count] : longest;
+        if (++count == REORDER_TENSORS) launch();
+      }
+    }
+    launch();
+    DA_CHECK_LAUNCH("state_reorder");
+  }
+  return 0;
+}

@@ -37,7 +37,8 @@ EXTRA_FLAGS = {"attn_prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "attn_both": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "attn_latent_mfma": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "attn_window": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "attn_f32": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+               "attn_f32": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "attn_beams": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 # Units whose kernels find their first arguments in registers when a wavefront starts: the hardware reads up to 14 words of them ahead,
 # as long as they are single numbers and pointers (a structure ends them).
 KERNARG_PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]

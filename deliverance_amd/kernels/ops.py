@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -184,6 +184,12 @@ _ARGTYPES = {
     "da_rglru_decode": [_VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, ctypes.c_long, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP],
     "da_rglru_portion": [_VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, ctypes.c_long, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I,
                          _VP, ctypes.c_long, _VP],
+    "da_beam_select_words": [_I, _I],
+    "da_beam_select": [_VP, ctypes.c_long, _I, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, ctypes.c_long, _VP],
+    "da_state_reorder": [_VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP],
+    "da_attn_beams_takes": [_I, _I],
+    "da_attn_beams_splits": [_I, _I, _I, _I, _I, _I, _I],
+    "da_attn_beams": [_VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP, _I, _I, _VP, ctypes.c_long, _VP],
 }
 _LIB = None
 
@@ -241,6 +247,14 @@ def _dev(*ts):
     for t in ts:
         if t is not None:
             _need(t.is_cuda, "kernel operands must live on the GPU")
+
+
+def _dev_here(*ts):
+    """``_dev``, and on the device whose current stream the launch goes to."""
+    _dev(*ts)
+    for t in ts:
+        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
+            raise KernelError(f"kernel operands lie on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _rows_2d(t: torch.Tensor, name: str):
@@ -335,6 +349,41 @@ def state_scatter(state: torch.Tensor, state_slots: torch.Tensor, q_start: torch
           and q_start.numel() >= n_seqs + 1, "state_scatter: slots [S] and q_start [S+1] must be int32")
     _check(_lib().da_state_scatter(_ptr(state), _ptr(state_slots), _ptr(q_start), _ptr(rows), n_seqs, state.shape[0],
                                    row_bytes, _stream()))
+
+
+def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor, dim: int = 0) -> Sequence[torch.Tensor]:
+    """In every tensor and every group g: row slots[g, b] becomes what row slots[g, parents[g, b]] was, in place; parents may be
+    any numbers 0 .. B - 1, in any order and with repeats.  ``slots`` and ``parents``: int32 [G, B] on the device, the slots distinct;
+    a place whose slot is no row (negative, say) or whose parent is outside 0 .. B - 1 is left as it is.
+    The rows lie along dimension ``dim``: tensors [rows, ...], or, with 1, [layers, rows, ...].  They must be contiguous, have equally
+    many rows of whole 4-byte words, and share no memory."""
+    _dev_here(slots, parents, *tensors)
+    _need(slots.dtype == parents.dtype == torch.int32 and slots.dim() == 2 and slots.shape == parents.shape and slots.is_contiguous()
+          and parents.is_contiguous(), "state_reorder: slots and parents must be contiguous int32 [groups, places]")
+    G, B = slots.shape
+    _need(1 <= B <= MAX_BEAMS, f"state_reorder: {B} places a group (1 to {MAX_BEAMS})")
+    _need(dim in (0, 1), "state_reorder: rows along dimension 0 or 1")
+    n = len(tensors)
+    if n == 0:
+        return tensors
+    pool = tensors[0].shape[dim] if tensors[0].dim() > dim else -1
+    ptrs, row_bytes, layers, spans = (ctypes.c_void_p * n)(), (ctypes.c_long * n)(), (ctypes.c_int * n)(), []
+    for i, t in enumerate(tensors):
+        if t.dim() <= dim or t.shape[dim] != pool or not t.is_contiguous():
+            raise KernelError(f"state_reorder: tensor {i} is {list(t.shape)}: contiguous tensors with {pool} rows along dimension {dim} are needed")
+        size = t.numel() * t.element_size()
+        ptrs[i], layers[i] = _ptr(t), t.shape[0] if dim else 1
+        row_bytes[i] = size // max(1, pool * layers[i])
+        if size and (row_bytes[i] == 0 or row_bytes[i] % 4):
+            raise KernelError(f"state_reorder: a row of tensor {i} has {row_bytes[i]} bytes, whole 4-byte words are needed")
+        if size == 0:
+            layers[i], row_bytes[i] = 0, 4
+        spans.append((t.data_ptr(), size))
+    spans.sort()
+    _need(all(a + size <= b for (a, size), (b, _) in zip(spans, spans[1:])), "state_reorder: two tensors share memory")
+    with _timed("state_reorder", 2 * G * B * sum(r * k for r, k in zip(row_bytes, layers)) if KernelProfiler.enabled else 0, 0, "fp32"):
+        _check(_lib().da_state_reorder(ptrs, row_bytes, layers, n, pool, _ptr(slots), _ptr(parents), G, B, _stream()))
+    return tensors
 
 
 # ------------------------------------------------------------------------------- norms
@@ -787,6 +836,43 @@ def sample(logits: torch.Tensor, params: torch.Tensor, out_tokens: torch.Tensor)
     return out_tokens
 
 
+MAX_BEAMS, MAX_CANDIDATES = 64, 128     # of a group (csrc/beam_select.hip)
+
+
+def beam_select_floats(n_rows: int, vocab: int) -> int:
+    """32-bit words of scratch that ``beam_select`` needs for logits [n_rows, vocab]."""
+    n = int(_lib().da_beam_select_words(int(n_rows), int(vocab)))
+    _need(n >= 0, f"beam_select: {n_rows} rows of {vocab} logits are too many")
+    return n
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_parents: torch.Tensor,
+                out_tokens: torch.Tensor, workspace: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The choice of beam search: rows g * n_beams + b of ``logits`` (float32) are the beams of group g, ``scores`` (float32, one a
+    row) their summed log-probabilities.  Of every group the K = out_scores.shape[1] pairs (beam, token) with the largest
+    score + log-probability go to ``out_scores`` (float32), ``out_parents`` and ``out_tokens`` (int32), all [G, K], in descending order,
+    the lowest beam and then the lowest token first among equals.  A score of -inf marks a place without a beam, a logit of -inf a
+    token that must not be chosen (no number counts as -inf in both); candidates that do not exist are (-inf, -1, -1).
+    ``workspace``: float32, ``beam_select_floats`` elements."""
+    _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace)
+    _rows_2d(logits, "logits")
+    R, V = logits.shape
+    _need(logits.dtype == scores.dtype == torch.float32, "beam_select: logits and scores must be float32")
+    _need(1 <= n_beams <= MAX_BEAMS and R % n_beams == 0, f"beam_select: {R} rows in groups of {n_beams} (1 to {MAX_BEAMS})")
+    G = R // n_beams
+    _need(scores.is_contiguous() and scores.numel() == R, "beam_select: one score a row")
+    K = out_scores.shape[-1]
+    _need(1 <= K <= MAX_CANDIDATES, f"beam_select: {K} candidates (1 to {MAX_CANDIDATES})")
+    for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32)):
+        if t.dtype != dtype or tuple(t.shape) != (G, K) or not t.is_contiguous():
+            raise KernelError(f"beam_select: outputs must be contiguous [{G}, {K}], float32 scores and int32 parents and tokens")
+    _need(workspace.dtype == torch.float32 and workspace.is_contiguous(), "beam_select: the workspace must be contiguous float32")
+    with _timed("beam_select", 4 * R * V, 4 * R * V, "fp32"):
+        _check(_lib().da_beam_select(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), K, _ptr(out_scores), _ptr(out_parents),
+                                     _ptr(out_tokens), _ptr(workspace), workspace.numel(), _stream()))
+    return out_scores, out_parents, out_tokens
+
+
 def top_logprobs(logits: torch.Tensor, params: torch.Tensor, n: int, out_idx: torch.Tensor,
                  out_lp: torch.Tensor) -> None:
     _dev(logits, params, out_idx, out_lp)
@@ -1233,6 +1319,46 @@ def attention_decode(q: torch.Tensor, cache_slot: torch.Tensor, block_table: tor
 
 def decode_workspace_floats(n_seqs: int, n_heads: int, head_dim: int, n_splits: int) -> int:
     return n_seqs * n_heads * n_splits * (head_dim + 2)
+
+
+def attention_beams_takes(head_dim: int, page: int) -> bool:
+    """Whether ``attention_beams`` takes these sizes."""
+    return bool(_lib().da_attn_beams_takes(int(head_dim), int(page)))
+
+
+def beam_splits(n_groups: int, n_beams: int, n_heads: int, n_kv_heads: int, head_dim: int, max_blocks: int, page: int) -> int:
+    """How many workgroups share a group's positions in ``attention_beams`` (1: none do).  The library's rule, from the step's shape
+    only, so that a recorded step keeps it."""
+    return int(_lib().da_attn_beams_splits(n_groups, n_beams, n_heads, n_kv_heads, head_dim, max_blocks, page))
+
+
+def beam_workspace_floats(n_seqs: int, n_heads: int, head_dim: int, n_splits: int) -> int:
+    return n_seqs * n_heads * n_splits * (head_dim + 2) if n_splits > 1 else 0
+
+
+def attention_beams(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, shared: torch.Tensor,
+                    n_beams: int, n_heads: int, scale: float, window: Optional[int], out: torch.Tensor, n_splits: int = 1,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_decode`` (bfloat16 or float32) of sequences in groups: rows g * n_beams + b of q, out, ``block_table`` and ``seq_lens``
+    are the beams of group g, and the tables of a group begin with the same pages: those of its first ``shared[g]`` positions
+    (int32 [G]; 0: none) are read once for all of them.  Lengths may differ; a sequence of length 0 gets zeros.  With ``n_splits`` > 1
+    a group's positions are shared out over that many workgroups, whose partial results pass through ``workspace`` (float32,
+    ``beam_workspace_floats`` elements)."""
+    _dev_here(q, cache_slot, block_table, seq_lens, shared, out, workspace)
+    Hkv, page, D = _attn_common(q, cache_slot, block_table, n_heads, out, "attention_beams", q.dtype)
+    S = seq_lens.numel()
+    _need(1 <= n_beams <= MAX_BEAMS and S % n_beams == 0, f"attention_beams: {S} sequences in groups of {n_beams} (1 to {MAX_BEAMS})")
+    G = S // n_beams
+    _need(q.shape[0] == S and out.shape[0] == S and block_table.shape[0] >= S, "attention_beams: q, out and block_table must have a row a sequence")
+    _need(seq_lens.dtype == shared.dtype == torch.int32 and seq_lens.is_contiguous() and shared.is_contiguous() and shared.numel() == G,
+          "attention_beams: seq_lens must be int32 [groups * beams], shared int32 [groups]")
+    _need(n_splits <= 1 or (workspace is not None and workspace.dtype == torch.float32 and workspace.is_contiguous()),
+          "attention_beams: more than one share needs a contiguous float32 workspace")
+    _check(_lib().da_attn_beams(_ptr(q), q.stride(0), _ptr(cache_slot), _dt(q), _ptr(block_table), block_table.shape[1], _ptr(seq_lens),
+                                _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), int(window or 0), _ptr(out), out.stride(0),
+                                max(1, int(n_splits)), _ptr(workspace) if n_splits > 1 else None, workspace.numel() if n_splits > 1 else 0,
+                                _stream()))
+    return out
 
 
 def attention_prefill(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torch.Tensor,
