@@ -16,11 +16,14 @@ between requests.  Here a pool of fixed size serves all requests:
 * ``extend`` reserves pages for a request's next tokens (all groups or nothing);
   ``commit`` makes them part of the request and returns pages that a window has passed;
   ``close`` returns everything.
+* ``fork`` makes a request that continues another one: full pages are held by both (a page goes
+  back when nobody holds it any more), the page that is being written is the new request's own.
+  ``reorder`` lets requests of one length (the beams of a search) continue one another, in place.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, Hashable, List, Optional, Sequence, Set, Tuple
 
 import numpy as np
 
@@ -54,8 +57,8 @@ class StateSpec:
 
 
 class PagePool:
-    """Page ids 0..n-1 with an owner each; free ids are handed out lowest first after reuse
-    in last-freed-first order."""
+    """Page ids 0..n-1 with an owner each, or several holders; free ids are handed out lowest first
+    after reuse in last-freed-first order."""
 
     def __init__(self, n_pages: int):
         if n_pages < 0:
@@ -63,6 +66,7 @@ class PagePool:
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, -1, -1))
         self._owner: List[Optional[Hashable]] = [None] * n_pages
+        self._holders: Dict[int, Set[Hashable]] = {}      # of the pages that more than one holds
 
     @property
     def n_free(self) -> int:
@@ -78,16 +82,42 @@ class PagePool:
             self._owner[p] = owner
         return out
 
-    def give(self, pages: Sequence[int], owner: Hashable) -> None:
+    def share(self, pages: Sequence[int], owner: Hashable) -> None:
+        """``owner`` holds these pages too; they are free again once every holder has given them back."""
+        if owner is None:
+            raise CacheError("pages need an owner")
+        for p in pages:
+            if p < 0 or p >= self.n_pages or self._owner[p] is None:
+                raise CacheError(f"page {p} is nobody's")
+            if self.held_by(p, owner):
+                raise CacheError(f"page {p} is held by {owner!r} already")
+            self._holders.setdefault(p, {self._owner[p]}).add(owner)
+
+    def held_by(self, page: int, owner: Hashable) -> bool:
+        return owner in self._holders[page] if page in self._holders else self._owner[page] == owner
+
+    def give(self, pages: Sequence[int], owner: Hashable) -> List[int]:
+        """Returns the pages that are free now (those that somebody else holds are not)."""
+        freed = []
         for p in pages:
             if p < 0 or p >= self.n_pages:
                 raise CacheError(f"page {p} is not in the pool")
             if self._owner[p] is None:
                 raise CacheError(f"page {p} freed twice")
-            if self._owner[p] != owner:
+            if not self.held_by(p, owner):
                 raise CacheError(f"page {p} belongs to {self._owner[p]!r}, not to {owner!r}")
+            holders = self._holders.get(p)
+            if holders is not None:
+                holders.remove(owner)
+                if self._owner[p] == owner:
+                    self._owner[p] = next(iter(holders))
+                if len(holders) == 1:
+                    del self._holders[p]
+                continue
             self._owner[p] = None
             self._free.append(p)
+            freed.append(p)
+        return freed
 
     def owner_of(self, page: int):
         return self._owner[page]
@@ -199,10 +229,11 @@ class CacheManager:
         r.pending += n_new
         return start
 
-    def _give(self, group: int, pages: Sequence[int], rid) -> None:
-        self.pools[group].give(pages, rid)
-        if pages and self.on_release is not None:
-            self.on_release(group, pages)
+    def _give(self, group: int, pages: Sequence[int], rid) -> List[int]:
+        freed = self.pools[group].give(pages, rid)
+        if freed and self.on_release is not None:
+            self.on_release(group, freed)
+        return freed
 
     def commit(self, rid, n: Optional[int] = None) -> List[Tuple[int, int]]:
         """The reserved positions (the first ``n`` of them, when given: a later step may have
@@ -221,8 +252,7 @@ class CacheManager:
             kept = -(-max(0, self.groups[g].keep_first) // self.page_size)   # pages of the first tokens stay
             for j in range(kept, min(first, len(t))):
                 if t[j] >= 0:
-                    self._give(g, [t[j]], rid)
-                    released.append((g, t[j]))
+                    released += [(g, p) for p in self._give(g, [t[j]], rid)]
                     t[j] = -1
         return released
 
@@ -248,6 +278,53 @@ class CacheManager:
             self._slot_owner[r.state_slot] = None
             self._free_slots.append(r.state_slot)
         del self._reqs[rid]
+
+    # ---- requests that continue one another ---------------------------------------------------
+    def writing(self, rid, group: int) -> int:
+        """The page that holds the request's last positions and has room for the next; -1 when the next
+        position begins a page."""
+        r = self._req(rid)
+        return r.tables[group][r.length // self.page_size] if r.length % self.page_size else -1
+
+    def fork(self, rid: Hashable, new: Hashable) -> None:
+        """Start a request that continues ``rid`` where it stands.  Full pages are shared; the page that is being written
+        (``writing``) and the state slot are the new request's own, and whoever holds the tensors fills them with what ``rid``'s
+        hold.  Either everything is there or nothing changes."""
+        r = self._req(rid)
+        if r.pending:
+            raise CacheError(f"request {rid!r} has positions reserved")
+        full, part = divmod(r.length, self.page_size)
+        if part and any(p.n_free < 1 for p in self.pools):
+            raise OutOfPages(f"request {new!r} needs a page per group, free: {[p.n_free for p in self.pools]}")
+        self.open(new)
+        n = self._reqs[new]
+        n.length = r.length
+        for g, pool in enumerate(self.pools):
+            shared = r.tables[g][:full]
+            pool.share([p for p in shared if p >= 0], new)
+            n.tables[g] = shared + (pool.take(1, new) if part else [])
+
+    def reorder(self, rids: Sequence[Hashable], parents: Sequence[int]) -> None:
+        """Request rids[i] continues what rids[parents[i]] was, for all i at once; they have one length and nothing reserved.  Full
+        pages are shared; every request keeps its own page that is being written and its own state slot, and whoever holds
+        the tensors reorders what these hold (``kernels.ops.state_reorder``)."""
+        reqs = [self._req(rid) for rid in rids]
+        if len(set(rids)) != len(reqs) or len(parents) != len(reqs) or any(not 0 <= p < len(reqs) for p in parents):
+            raise CacheError(f"parents {list(parents)} of {len(reqs)} requests")
+        if any(r.pending or r.length != reqs[0].length for r in reqs):
+            raise CacheError("requests that continue one another have one length and nothing reserved")
+        full = reqs[0].length // self.page_size if reqs else 0
+        for g, pool in enumerate(self.pools):
+            old = [r.tables[g] for r in reqs]
+            new = [t if p == i else old[p][:full] + t[full:] for i, (t, p) in enumerate(zip(old, parents))]
+            for rid, before, after in zip(rids, old, new):        # everybody takes before anybody gives
+                if after is not before:
+                    pool.share([p for p in after[:full] if p >= 0 and not pool.held_by(p, rid)], rid)
+            for rid, r, before, after in zip(rids, reqs, old, new):
+                if after is not before:
+                    r.tables[g] = after
+                    keep = set(after)
+                    self._give(g, [p for p in before if p >= 0 and p not in keep], rid)
 
     # ---- addressing --------------------------------------------------------------
     def slots_for(self, rid, group: int, start: int, n: int) -> List[int]:
@@ -277,15 +354,18 @@ class CacheManager:
                 for p in r.tables[g]:
                     if p < 0:
                         continue
-                    if p in held:
-                        raise CacheError(f"group {g}: page {p} held by {held[p]!r} and {rid!r}")
-                    held[p] = rid
-                    if pool.owner_of(p) != rid:
+                    if p in held and p not in pool._holders:
+                        raise CacheError(f"group {g}: page {p} held by {held[p][0]!r} and {rid!r}")
+                    held.setdefault(p, []).append(rid)
+                    if not pool.held_by(p, rid):
                         raise CacheError(f"group {g}: page {p} in the table of {rid!r} but owned by {pool.owner_of(p)!r}")
                 want = -(-(r.length + r.pending) // self.page_size)
                 if len(r.tables[g]) != want:
                     raise CacheError(f"group {g}: table of {rid!r} has {len(r.tables[g])} entries for "
                                      f"{r.length + r.pending} positions")
+            for p, holders in pool._holders.items():
+                if len(holders) < 2 or holders != set(held.get(p, [])):
+                    raise CacheError(f"group {g}: page {p} counted for {holders!r}, in the tables of {held.get(p)!r}")
             free = pool._free
             if len(set(free)) != len(free):
                 raise CacheError(f"group {g}: a page is on the free list twice")

@@ -1,0 +1,211 @@
+"""Beam search's host side (no GPU): requests that continue one another in the cache manager, and the search for one prompt."""
+import math
+import random
+
+import numpy as np
+import pytest
+
+import plain_beams
+from deliverance_amd.cache import CacheError, CacheManager, KVGroupSpec, OutOfPages, PagePool, StateSpec
+
+
+def manager(pages=40, slots=0, window=None):
+    return CacheManager([KVGroupSpec((0, 1), 2, 16, None), KVGroupSpec((2,), 2, 16, window)], 4, [pages, pages], [StateSpec(3, 5)] if slots else [], slots)
+
+
+def test_shared_pages_go_back_with_their_last_holder():
+    p = PagePool(3)
+    a = p.take(2, "a")
+    p.share(a, "b")
+    p.share([a[0]], "c")
+    with pytest.raises(CacheError, match="already"):
+        p.share([a[0]], "c")
+    with pytest.raises(CacheError, match="nobody's"):
+        p.share([2], "b")
+    with pytest.raises(CacheError, match="belongs to"):
+        p.give([a[1]], "c")
+    assert p.give(a, "a") == [] and p.n_free == 1
+    assert p.owner_of(a[1]) == "b" and not p.held_by(a[0], "a")
+    assert p.give([a[1]], "b") == [a[1]] and p.give([a[0]], "c") == [] and p.give([a[0]], "b") == [a[0]]
+    with pytest.raises(CacheError, match="freed twice"):
+        p.give([a[0]], "b")
+    assert p.n_free == 3 and p._holders == {}
+
+
+def test_a_fork_shares_full_pages_and_writes_its_own():
+    m = manager(slots=3)
+    m.open("a")
+    m.extend("a", 10)
+    with pytest.raises(CacheError, match="reserved"):
+        m.fork("a", "b")
+    m.commit("a")
+    m.fork("a", "b")
+    m.check()
+    assert m.length("b") == 10 and m.table("b", 0)[:2] == m.table("a", 0)[:2] and m.table("b", 0)[2] != m.table("a", 0)[2]
+    assert m.writing("a", 0) == m.table("a", 0)[2] and m.state_slot("a") != m.state_slot("b")
+    freed = []
+    m.on_release = lambda g, pages: freed.extend((g, p) for p in pages)
+    shared, own = m.table("a", 0)[:2], m.table("a", 0)[2]
+    m.close("a")
+    assert (0, own) in freed and not any((0, p) in freed for p in shared)
+    m.check()
+    m.close("b")
+    m.check()
+    assert m.stats()["pages_free"] == [40, 40] and m.stats()["state_slots_free"] == 3
+
+
+def test_a_fork_at_a_pages_end_takes_no_page():
+    m = manager(pages=2)
+    m.open("a")
+    m.extend("a", 8)
+    m.commit("a")
+    m.fork("a", "b")
+    assert m.table("b", 0) == m.table("a", 0) and m.writing("b", 0) == -1
+    with pytest.raises(OutOfPages):
+        m.extend("b", 1)
+    m.check()
+
+
+def test_a_fork_that_does_not_fit_changes_nothing():
+    m = manager(pages=3)
+    m.open("a")
+    m.extend("a", 9)
+    m.commit("a")
+    with pytest.raises(OutOfPages):
+        m.fork("a", "b")
+    assert m.live() == ["a"]
+    m.check()
+
+
+@pytest.mark.parametrize("window", [None, 5])
+@pytest.mark.parametrize("seed", range(6))
+def test_tables_follow_their_parents(seed, window):
+    """Random searches against a plain record of what every beam's positions are.  A page stands for the contents written there; the
+    page that is being written is copied as the device does it."""
+    rng = random.Random(seed)
+    m = manager(pages=200, slots=8, window=window)
+    B = rng.randint(2, 5)
+    rids, rows, plain = [f"b{i}" for i in range(B)], [{}, {}], [[] for _ in range(B)]
+    m.on_release = lambda g, pages: [rows[g].pop((p, i), None) for p in pages for i in range(4)]
+
+    def write(rid, k, values):
+        start = m.extend(rid, len(values))
+        for g in (0, 1):
+            for i, s in enumerate(m.slots_for(rid, g, start, len(values))):
+                rows[g][(s // 4, s % 4)] = values[i]
+        plain[k] += values
+
+    m.open(rids[0])
+    write(rids[0], 0, [rng.random() for _ in range(rng.randint(1, 9))])
+    m.commit(rids[0])
+    for r in rids[1:]:
+        m.fork(rids[0], r)
+
+    def reorder(parents):
+        old = [[m.writing(r, g) for r in rids] for g in (0, 1)]
+        m.reorder(rids, parents)
+        for g in (0, 1):
+            assert [m.writing(r, g) for r in rids] == old[g], "everyone keeps the page that it writes"
+            before = dict(rows[g])
+            for b, p in enumerate(parents):
+                for i in range(4):
+                    if old[g][b] >= 0 and (old[g][p], i) in before:
+                        rows[g][(old[g][b], i)] = before[(old[g][p], i)]
+        plain[:] = [list(plain[p]) for p in parents]
+
+    reorder([0] * B)
+    for step in range(25):
+        for k, r in enumerate(rids):
+            write(r, k, [rng.random()])
+            m.commit(r)
+        reorder([rng.randrange(B) for _ in range(B)])
+        m.check()
+        for k, r in enumerate(rids):
+            n = m.length(r)
+            assert n == len(plain[k])
+            for g in (0, 1):
+                for pos in range(0 if g == 0 or window is None else max(0, n - window + 1), n):
+                    assert rows[g][(m.table(r, g)[pos // 4], pos % 4)] == plain[k][pos], (step, k, g, pos)
+    for r in rids:
+        m.close(r)
+    m.check()
+    assert m.stats()["pages_free"] == [200, 200]
+
+
+def test_refusals_of_the_manager():
+    m = manager()
+    for r in "ab":
+        m.open(r)
+        m.extend(r, 3)
+        m.commit(r)
+    for rids, parents in ((["a", "b"], [0]), (["a", "b"], [0, 2]), (["a", "a"], [0, 0]), (["a", "b"], [-1, 0])):
+        with pytest.raises(CacheError):
+            m.reorder(rids, parents)
+    m.extend("b", 1)
+    with pytest.raises(CacheError, match="one length"):
+        m.reorder(["a", "b"], [0, 0])
+    m.commit("b")
+    with pytest.raises(CacheError, match="one length"):
+        m.reorder(["a", "b"], [0, 0])
+
+
+def group_search(logits_of, prompt, n_beams, max_new, ends=(), **options):
+    """The search through ``BeamGroup``, with the choice made here."""
+    from deliverance_amd.engine.beams import BeamGroup, BeamParameters
+    p = BeamParameters(num_beams=n_beams, max_tokens=max_new, **options)
+    p.validate(len(ends))
+    g = BeamGroup(p, ends, max_new)
+    while not g.done:
+        found = []
+        for b, (score, tokens) in enumerate(zip(g.scores, g.tokens)):
+            if score == -math.inf:
+                continue
+            z = np.asarray(logits_of(list(prompt) + tokens), dtype=np.float64)
+            z = z - z.max()
+            z = z - math.log(np.exp(z).sum())
+            found += [(score + z[v], b, v) for v in range(len(z))]
+        found.sort(key=lambda c: (-c[0], c[1], c[2]))
+        found = found[:p.candidates(len(ends))]
+        found += [(-math.inf, -1, -1)] * (p.candidates(len(ends)) - len(found))
+        before = list(g.tokens)
+        parents = g.take(found)
+        if not g.done:
+            chosen = {q for s, q in zip(g.scores, parents) if s > -math.inf}
+            assert all(parents[q] == q for q in chosen), "a beam that goes on keeps its place"
+            for b, q in enumerate(parents):
+                assert g.tokens[b][:-1] == before[q]
+    return g.finished
+
+
+@pytest.mark.parametrize("seed", range(8))
+@pytest.mark.parametrize("options", [{}, {"length_penalty": 0.0}, {"length_penalty": 2.0, "early_stopping": True}])
+def test_the_search_is_the_plain_one(seed, options):
+    vocab, n_beams, max_new = [3, 7, 12, 30][seed % 4], 1 + seed % 5, 2 + seed
+    ends = () if seed % 3 == 0 else tuple(range(seed % 3))
+
+    def logits_of(ids):
+        return np.random.default_rng([seed, *ids]).normal(size=vocab) * 2
+
+    want, gap = plain_beams.beam_search(logits_of, [5, 1], n_beams, max_new, ends, **options)
+    got = group_search(logits_of, [5, 1], n_beams, max_new, ends, **options)
+    assert gap > 0
+    assert [(h.tokens, h.finish_reason) for h in got] == [(t, "stop" if t[-1] in ends else "length") for _, _, t in want]
+    assert np.allclose([h.score for h in got], [s for _, s, _ in want])
+
+
+def test_refusals_of_the_parameters():
+    from deliverance_amd.engine.beams import BeamParameters
+    BeamParameters().validate(1)
+    for bad in (dict(num_beams=0), dict(num_beams=65), dict(max_tokens=0), dict(ntokens=0), dict(length_penalty=math.nan)):
+        with pytest.raises(ValueError):
+            BeamParameters(**bad).validate(1)
+    with pytest.raises(ValueError, match="candidates"):
+        BeamParameters(num_beams=60).validate(2)
+    BeamParameters(num_beams=60, ignore_eos=True).validate(2)
+
+
+def test_shared_scores_and_positions_of_a_padded_step():
+    from deliverance_amd.engine.step import BeamStep, StepRunner
+    words = StepRunner._beam_words(BeamStep(2, 4, [-1.5, -math.inf], [[32], [16]]), 2)
+    assert np.array(words[:4], dtype=np.int32).view(np.float32).tolist() == [-1.5, -math.inf, -math.inf, -math.inf]
+    assert words[4:] == [32, 0, 16, 0]
