@@ -17,6 +17,9 @@ def __getattr__(name):
     if name in ("AutoModelForCausalLM", "CausalLanguageModel", "Response"):
         from .engine import engine as _e
         return getattr(_e, name)
+    if name in ("BeamParameters", "BeamHypothesis", "BeamResponse"):
+        from .engine import beams as _b
+        return getattr(_b, name)
     if name == "random_model":
         from .random_model import random_model
         return random_model
@@ -24,4 +27,4 @@ def __getattr__(name):
 
 
 __all__ = ["AutoModelForCausalLM", "CausalLanguageModel", "Response", "GeneratorParameters", "EngineConfig",
-           "Gpt2Config", "ModelSupport", "Architecture", "random_model"]
+           "Gpt2Config", "ModelSupport", "Architecture", "random_model", "BeamParameters", "BeamHypothesis", "BeamResponse"]

@@ -60,6 +60,8 @@ def cmd_generate(a) -> int:
         InferenceProfiler.enable(sync=True)
         KernelProfiler.enable()            # every kernel launch timed on the device (no recorded graphs meanwhile)
     model = AutoModelForCausalLM.from_pretrained(a.model, engine_config=EngineConfig(**cfg))
+    if a.num_beams is not None:
+        return _beam_search(a, model, prompts)
     params = GeneratorParameters(temperature=a.temperature, seed=a.seed, max_tokens=a.max_tokens, ntokens=a.ntokens,
                                  top_k=a.top_k, top_p=a.top_p, uniform_top_p=a.uniform_top_p,
                                  xtc_threshold=a.xtc_threshold, xtc_probability=a.xtc_probability,
@@ -101,6 +103,38 @@ def cmd_generate(a) -> int:
         print(InferenceProfiler.summary("(stages drained at their end)"), file=sys.stderr)
         print(KernelProfiler.summary("(device time per kernel against what it must move and compute; % of 8 TB/s or of "
                                      "the matrix peak, whichever binds)"), file=sys.stderr)
+    return 0
+
+
+def _beam_search(a, model, prompts) -> int:
+    """The best hypothesis of every prompt on stdout, all of them in the JSONL file."""
+    from .engine.beams import BeamParameters
+    params = BeamParameters(num_beams=a.num_beams, max_tokens=a.max_tokens, ntokens=a.ntokens, length_penalty=a.length_penalty,
+                            early_stopping=a.early_stopping, ignore_eos=a.ignore_eos)
+    for p in prompts[:a.warmup_cases]:
+        model.beam_search(p, params)
+    t0 = time.perf_counter()
+    outs = model.beam_search(prompts, params) if a.batch else [model.beam_search(p, params) for p in prompts]
+    wall = time.perf_counter() - t0
+    rows = []
+    for p, r in zip(prompts, outs):
+        best = r.hypotheses[0] if r.hypotheses else None
+        print(f"beam_search_complete prompt_tokens={r.prompt_tokens} hypotheses={len(r.hypotheses)} generated_tokens={len(r.generated_tokens)} "
+              f"score={best.score if best else 0:.4f} total_ms={r.total_time_ms:.3f} finish_reason={best.finish_reason if best else 'error'}", file=sys.stderr)
+        print(",".join(str(t) for t in r.generated_tokens))
+        rows.append(dict(prompt_ids=p, prompt_tokens=r.prompt_tokens, total_ms=round(r.total_time_ms, 3), generated_tokens=len(r.generated_tokens),
+                         hypotheses=[dict(token_ids=h.tokens, score=h.score, rank=h.rank, finish_reason=h.finish_reason) for h in r.hypotheses]))
+    print(f"requests={len(rows)} num_beams={a.num_beams} wall_s={wall:.3f}", file=sys.stderr)
+    if a.output:
+        with open(a.output, "w", newline="") as f:
+            w = csv.writer(f)
+            w.writerow(["prompt_tokens", "generated_tokens", "total_ms"])
+            for r in rows:
+                w.writerow([r[k] for k in ("prompt_tokens", "generated_tokens", "total_ms")])
+    if a.jsonl_output:
+        with open(a.jsonl_output, "w") as f:
+            for r in rows:
+                f.write(json.dumps(r) + "\n")
     return 0
 
 
@@ -158,6 +192,9 @@ def main(argv=None) -> int:
     g.add_argument("--xtc-threshold", type=float, default=None)
     g.add_argument("--xtc-probability", type=float, default=None)
     g.add_argument("--ignore-eos", action="store_true")
+    g.add_argument("--num-beams", type=int, default=None, help="beam search with so many beams in place of sampling")
+    g.add_argument("--length-penalty", type=float, default=1.0, help="beam search: hypotheses are ranked by score / length ** this, default 1.0")
+    g.add_argument("--early-stopping", action="store_true", help="beam search: a prompt ends with its first num-beams finished hypotheses")
     g.add_argument("--warmup-cases", type=int, default=1, help="prompts to run before recording, default 1")
     g.add_argument("--max-cases", type=int, default=None)
     g.add_argument("--kv-context-rows-per-page", type=int, default=None, help="tokens per cache page, default 16")

@@ -13,7 +13,7 @@
 
 struct ReorderTable {
   void* data[REORDER_TENSORS];
-  int units[REORDER_TENSORS];    // of a row: 16 bytes each (WIDE) or 4
+  int units[REORDER_TENSORS];    // of a row, 16, 4 or 2 bytes each
 };
 
 // NB: places that a thread has registers for
@@ -43,35 +43,39 @@ reorder_kernel(const ReorderTable table, const int* __restrict__ slots, const in
     if (to[b] >= 0) data[(size_t)to[b] * units + c] = v[b];
 }
 
-// n tensors [layers, pool, row]; `data`, `row_bytes` (whole 4-byte words) and `layers` are host arrays.
+// n tensors [layers, pool, row]; `data`, `row_bytes` (even) and `layers` are host arrays.
 extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const int* layers, int n, int pool, const int* slots,
                                 const int* parents, int G, int B, void* stream) {
   DA_REQUIRE(n >= 0 && G >= 0 && G <= 65535 && B > 0 && B <= REORDER_MAX && pool >= 0,
              "state_reorder: bad sizes (tensors=%d rows=%d groups=%d places=%d; at most %d places)", n, pool, G, B, REORDER_MAX);
   for (int i = 0; i < n; ++i)
-    DA_REQUIRE(row_bytes[i] > 0 && row_bytes[i] % 4 == 0 && row_bytes[i] < (1L << 32) && (uintptr_t)data[i] % 4 == 0 && layers[i] >= 0,
-               "state_reorder: %d layers with a row of %ld bytes: not whole words, or too long", layers[i], row_bytes[i]);
+    DA_REQUIRE(row_bytes[i] > 0 && row_bytes[i] % 2 == 0 && row_bytes[i] < (1L << 31) && (uintptr_t)data[i] % 2 == 0 && layers[i] >= 0,
+               "state_reorder: %d layers with a row of %ld bytes: not whole 2-byte units, or too long", layers[i], row_bytes[i]);
   if (n == 0 || G == 0 || B == 1 || pool == 0) return 0;
-  auto is_wide = [&](int i) { return B <= 16 && row_bytes[i] % 16 == 0 && (uintptr_t)data[i] % 16 == 0; };
-  for (int wide = 0; wide < 2; ++wide) {
+  auto unit_of = [&](int i) {
+    const uintptr_t odd = (uintptr_t)data[i] | (uintptr_t)row_bytes[i];
+    return B <= 16 && odd % 16 == 0 ? 16 : (odd % 4 == 0 ? 4 : 2);
+  };
+  for (int unit = 16; unit > 1; unit = unit == 16 ? 4 : unit - 2) {      // 16, 4, 2
     ReorderTable table;
     int count = 0, longest = 0;
     auto launch = [&]() {
       if (!count) return;
       const dim3 grid(da_ceil_div(longest, REORDER_THREADS), count, G), block(REORDER_THREADS);
       hipStream_t s = (hipStream_t)stream;
-      if (wide && B <= 4) hipLaunchKernelGGL((reorder_kernel<uint4, 4>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (wide && B <= 8) hipLaunchKernelGGL((reorder_kernel<uint4, 8>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (wide) hipLaunchKernelGGL((reorder_kernel<uint4, 16>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (B <= 16) hipLaunchKernelGGL((reorder_kernel<uint32_t, 16>), grid, block, 0, s, table, slots, parents, B, pool);
-      else hipLaunchKernelGGL((reorder_kernel<uint32_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
+      if (unit == 16 && B <= 4) hipLaunchKernelGGL((reorder_kernel<uint4, 4>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (unit == 16 && B <= 8) hipLaunchKernelGGL((reorder_kernel<uint4, 8>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (unit == 16) hipLaunchKernelGGL((reorder_kernel<uint4, 16>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (unit == 4 && B <= 16) hipLaunchKernelGGL((reorder_kernel<uint32_t, 16>), grid, block, 0, s, table, slots, parents, B, pool);
+      else if (unit == 4) hipLaunchKernelGGL((reorder_kernel<uint32_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
+      else hipLaunchKernelGGL((reorder_kernel<uint16_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
       count = longest = 0;
     };
     for (int i = 0; i < n; ++i) {
-      if ((int)is_wide(i) != wide) continue;
+      if (unit_of(i) != unit) continue;
       for (int layer = 0; layer < layers[i]; ++layer) {
         table.data[count] = (char*)data[i] + (long)layer * pool * row_bytes[i];
-        table.units[count] = (int)(row_bytes[i] / (wide ? 16 : 4));
+        table.units[count] = (int)(row_bytes[i] / unit);
         longest = table.units[count] > longest ? table.units[count] : longest;
         if (++count == REORDER_TENSORS) launch();
       }

@@ -26,6 +26,7 @@ from ..models.causal_lm import CausalLM, load_model
 from ..profiler import InferenceProfiler
 from ..sampling.params import GeneratorParameters
 from ..sampling.sampler import RECORD_WORDS, device_record
+from .beams import BeamParameters, BeamResponse, BeamSearch
 from .device_cache import DeviceCache
 from .scheduler import RUNNING, Request, Scheduled, Scheduler
 from .step import StepEntry, StepRunner
@@ -301,6 +302,18 @@ class CausalLanguageModel:
         out = [self._response(got[r]) for r in rids]
         for r in rids:
             self.scheduler.finished.remove(got[r])
+        return out[0] if single else out
+
+    def beam_search(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]],
+                    params: Optional[BeamParameters] = None) -> Union[BeamResponse, List[BeamResponse]]:
+        """The most likely continuations of one prompt (a list of token ids) or several (a list of lists), by beam search:
+        ``num_beams`` hypotheses a prompt, best first.  Prompts are searched side by side as far as the cache pool and
+        ``max_num_seqs`` allow.  The engine must have no other work meanwhile."""
+        single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple))
+        if self.has_work():
+            raise RuntimeError("beam search needs an engine without other requests")
+        build.ensure(["beam_select", "reorder", "attn_beams"])
+        out = BeamSearch(self.cache, self.runner, self.config, self.engine_config, params or BeamParameters()).run([prompts] if single else list(prompts))
         return out[0] if single else out
 
     @staticmethod

@@ -33,6 +33,15 @@ class StepEntry:
     from_sampled: Optional[int] = None
 
 
+@dataclass
+class BeamStep:
+    """What a step of beam search brings beside its entries, which are the beams of one request after another, one token each."""
+    n_beams: int                    # beams of a request
+    n_keep: int                     # candidates that are wanted of every request
+    scores: Sequence[float]         # the beams' summed log-probabilities, one an entry (-inf: no beam)
+    shared: Sequence[Sequence[int]]  # per cache group and request: positions in pages that all its beams have in common
+
+
 class StepError(ValueError):
     pass
 
@@ -46,12 +55,12 @@ class StepPacker:
         self.n_groups = n_groups
         self.page_size = page_size
 
-    def layout(self, entries, order, pad_to, max_blocks, extra):
+    def layout(self, entries, order, pad_to, max_blocks, extra, extra_a_pad=RECORD_WORDS):
         """Where each array of the step lies in its one buffer of integers: tokens, where a token
         comes from, positions, sequence ids, row starts, lengths, state slots, wanted rows, then
-        per cache group the cache row of every token and the block tables, then ``extra``.  With
-        ``pad_to`` the step is filled up with empty one-token sequences (length 0, no cache row),
-        so that its shape is fixed."""
+        per cache group the cache row of every token and the block tables, then ``extra`` (and
+        ``extra_a_pad`` zeros for each sequence that is filled up).  With ``pad_to`` the step is filled up with
+        empty one-token sequences (length 0, no cache row), so that its shape is fixed."""
         mgr = self.manager
         S_real = len(entries)
         n_pad = 0 if pad_to is None else pad_to - S_real
@@ -61,7 +70,7 @@ class StepPacker:
         G = self.n_groups
         if max_blocks is None:
             max_blocks = max(1, max(len(mgr.table(e.rid, g)) for e in entries for g in range(G))) if G else 1
-        n_extra = 0 if not extra else len(extra) + RECORD_WORDS * n_pad
+        n_extra = 0 if not extra else len(extra) + extra_a_pad * n_pad
         offs = {}
         o = 0
         for name, n in (("tokens", N), ("token_src", N), ("positions", N), ("seq_of", N), ("q_start", S + 1),
@@ -202,14 +211,16 @@ class StepRunner:
 
     # ---- the step --------------------------------------------------------------------------
     def run(self, entries: Sequence[StepEntry], reserved: bool = False,
-            sample_records: Optional[List[int]] = None):
+            sample_records: Optional[List[int]] = None, beams: Optional[BeamStep] = None):
         """Run one step.  Returns (logits [R, V] float32 on the device, ctx).  The rows follow
         the order of ``entries`` and of each entry's ``want``.  With ``reserved`` the caller has
         already opened the requests and reserved their positions (``CacheManager.extend``).
         ``sample_records`` (8 words per wanted row, see sampling.device_record) ride along in the
         same host-to-device copy (``ctx.extra``); when they are given and the step holds one-token
         sequences only, the step and its sampling are replayed from a recorded HIP graph and the
-        sampled tokens are left in ``ctx.sampled`` (the first rows of ``self.sampled``)."""
+        sampled tokens are left in ``ctx.sampled`` (the first rows of ``self.sampled``).  With ``beams`` (in place of
+        ``sample_records``) the step's entries are beams, one token each whose logits are wanted, and the choice of the next ones
+        (``ops.beam_select``) is left in ``ctx.chosen``: scores, parents and tokens, [requests, n_keep] each, on the device."""
         mgr = self.cache.manager
         cfg = self.model.config
         if not entries:
@@ -233,6 +244,14 @@ class StepRunner:
                     raise StepError(f"request {e.rid!r}: wanted place {w} is outside its {len(e.tokens)} tokens")
             if e.from_sampled is not None and not (len(e.tokens) == 1 and 0 <= e.from_sampled < self.sampled.numel()):
                 raise StepError(f"request {e.rid!r}: only a single token can come from the sampled tokens")
+
+        if beams is not None:
+            if sample_records is not None or any(len(e.tokens) != 1 or list(e.want) != [0] for e in entries):
+                raise StepError("beams bring one token each, whose logits are wanted, and no sampling records")
+            n = len(entries) // max(1, beams.n_beams)
+            if n * beams.n_beams != len(entries) or len(beams.scores) != len(entries) or \
+                    [len(p) for p in beams.shared] != [n] * len(self.cache.groups):
+                raise StepError(f"{len(entries)} entries, {len(beams.scores)} scores, groups of {beams.n_beams} beams")
 
         starts = {}
         opened = []
@@ -264,16 +283,16 @@ class StepRunner:
         order = sorted(range(len(entries)), key=lambda i: (len(entries[i].tokens) != 1, i))
         n_decode = sum(1 for e in entries if len(e.tokens) == 1)
         from ..profiler import KernelProfiler
-        graph_ok = (sample_records is not None and n_decode == len(entries) and self.use_graphs
+        graph_ok = ((sample_records is not None or beams is not None) and n_decode == len(entries) and self.use_graphs
                     and self.debug_hook is None and not KernelProfiler.enabled
                     and len(entries) <= self.max_graph_batch and all(list(e.want) == [0] for e in entries))
         from ..kernels import ops
         try:
             with ops.kernel_mode_scope(self.kernels):
                 if graph_ok:
-                    logits, ctx = self._run_graph(entries, starts, sample_records)
+                    logits, ctx = self._run_graph(entries, starts, sample_records, beams)
                 else:
-                    logits, ctx = self._run_eager(entries, order, starts, sample_records)
+                    logits, ctx = self._run_eager(entries, order, starts, sample_records, beams)
         except Exception:
             # A launch that was refused (a size no kernel takes) leaves nothing half-done on the host:
             # what this call reserved goes back, requests it opened are closed.  A caller that
@@ -289,27 +308,67 @@ class StepRunner:
                 mgr.commit(e.rid)
         return logits, ctx
 
-    def _run_eager(self, entries, order, starts, sample_records):
+    @staticmethod
+    def _beam_words(beams: BeamStep, n_requests: int) -> List[int]:
+        """The beams' scores (as the bits of 32-bit floats) and, per cache group, the shared positions, for ``n_requests``
+        requests, of which those behind the step's own are empty."""
+        n = n_requests * beams.n_beams
+        scores = np.full(n, -np.inf, dtype=np.float32)
+        scores[:len(beams.scores)] = beams.scores
+        words = scores.view(np.int32).tolist()
+        for per_request in beams.shared:
+            words += list(per_request) + [0] * (n_requests - len(per_request))
+        return words
+
+    def _take_beams(self, ctx, beams: BeamStep) -> None:
+        """Where the step's arrays of beam search lie in ``ctx.extra``."""
+        n, G = ctx.n_seqs, len(self.cache.groups)
+        per = n // beams.n_beams
+        ctx.n_beams = beams.n_beams
+        ctx.beam_scores = ctx.extra[:n].view(torch.float32)
+        ctx.beam_shared = [ctx.extra[n + g * per:n + (g + 1) * per] for g in range(G)]
+
+    def _choose(self, ctx, beams: BeamStep, logits: torch.Tensor):
         from ..kernels import ops
-        offs, meta, n_words = self._layout(entries, order, pad_to=None, max_blocks=None, extra=sample_records)
-        self._fill(self._staging_for(n_words), offs, meta, entries, order, starts, sample_records)
+        per = ctx.n_seqs // beams.n_beams
+        out = (ctx.buf("beam_out_scores", per, beams.n_keep, torch.float32), ctx.buf("beam_out_parents", per, beams.n_keep, torch.int32),
+               ctx.buf("beam_out_tokens", per, beams.n_keep, torch.int32))
+        ws = ctx.flat("beam_select", ops.beam_select_floats(*logits.shape), torch.float32)
+        return ops.beam_select(logits, ctx.beam_scores, beams.n_beams, *out, ws)
+
+    def _run_eager(self, entries, order, starts, sample_records, beams=None):
+        from ..kernels import ops
+        extra = sample_records if beams is None else self._beam_words(beams, len(entries) // beams.n_beams)
+        offs, meta, n_words = self._layout(entries, order, pad_to=None, max_blocks=None, extra=extra)
+        self._fill(self._staging_for(n_words), offs, meta, entries, order, starts, extra)
         dev = self._upload(n_words)
         ctx = self._context(dev, offs, meta, self.arena)
+        if beams is not None:
+            self._take_beams(ctx, beams)
         ctx.debug_hook = self.debug_hook
         self.last_ctx = ctx
         R = meta["R"]
         if any(e.from_sampled is not None for e in entries):
             ops.take_tokens(ctx.tokens, ctx.token_src, self.sampled, self.model.config.vocab_size)
         logits = self._forward(ctx, ctx.want_rows if R else None, R)
+        if beams is not None:
+            ctx.chosen = self._choose(ctx, beams, logits)
         return logits, ctx
 
     def _forward(self, ctx, want_rows, n_want):
         """The model's forward pass of this step: from C++ in one call, or part by part (always with the
         debug hook or the kernel profiler, which look between the kernels)."""
         from ..profiler import KernelProfiler
-        if self.native is not None and ctx.debug_hook is None and not KernelProfiler.enabled:
+        if self.native is not None and ctx.debug_hook is None and not KernelProfiler.enabled and not self._beams_attend(ctx):
             return self.native.forward(ctx, want_rows, n_want)
         return self.model.forward(ctx, want_rows, n_want)
+
+    def _beams_attend(self, ctx) -> bool:
+        """Whether attention of this step reads what beams share once (``ops.attention_beams``): the calls that are issued from C++
+        do not know of it."""
+        from ..kernels import ops
+        return ctx.n_beams > 1 and any(ops.attention_beams_pays(ctx, ctx.group_of(c.cache), blk.n_heads, blk.n_kv_heads, blk.head_dim, self.cache.page_size)
+                                       for c in self.model.config.schedule for blk in (self.model.blocks[c.layer].mixer,))
 
     def _context(self, dev, offs, meta, arena) -> StepContext:
         def view(name):
@@ -336,41 +395,48 @@ class StepRunner:
         return ctx
 
     # ---- decode-only steps replayed from a HIP graph ----------------------------------------------
-    def _run_graph(self, entries, starts, sample_records):
+    def _run_graph(self, entries, starts, sample_records, beams=None):
         """A step of one-token sequences only has a fixed shape once it is padded to a bucket
-        size, so its kernels (model and sampling) are recorded once per bucket and replayed.
-        Only the step's integers change: they are copied into the bucket's own buffer first."""
+        size, so its kernels (model and sampling, or the choice among beams) are recorded once per bucket and
+        replayed.  Only the step's integers change: they are copied into the bucket's own buffer first."""
         from ..kernels import ops
         S = len(entries)
-        bucket = 1
+        unit = 1 if beams is None else beams.n_beams       # (beams are padded request by request)
+        bucket = unit
         while bucket < S:
             bucket *= 2
         order = list(range(S))
-        offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap,
-                                           extra=sample_records)
-        st = self._graphs.get(bucket)
+        extra, a_pad = (sample_records, RECORD_WORDS) if beams is None else (self._beam_words(beams, bucket // unit), 0)
+        offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap, extra=extra, extra_a_pad=a_pad)
+        key = bucket if beams is None else (bucket, beams.n_beams, beams.n_keep)
+        st = self._graphs.get(key)
         if st is None:
             host = torch.empty(n_words, dtype=torch.int32, pin_memory=True)
             st = {"dev": torch.empty(n_words, dtype=torch.int32, device=self.device),
                   "host": host, "host_np": host.numpy(),
                   "arena": Arena(self.device), "graph": None, "copied": None}
-            self._graphs[bucket] = st
+            self._graphs[key] = st
         assert st["dev"].numel() == n_words, "a bucket's layout is fixed"
         if st["copied"] is not None:
             st["copied"].synchronize()
-        self._fill(st["host_np"], offs, meta, entries, order, starts, sample_records)
+        self._fill(st["host_np"], offs, meta, entries, order, starts, extra)
         st["dev"].copy_(st["host"], non_blocking=True)
         st["copied"] = torch.cuda.Event()
         st["copied"].record()
         ctx = self._context(st["dev"], offs, meta, st["arena"])
         self.last_ctx = ctx
+        if beams is not None:
+            self._take_beams(ctx, beams)
 
         sampled = self.sampled[:bucket]
 
         def body():
             ops.take_tokens(ctx.tokens, ctx.token_src, self.sampled, self.model.config.vocab_size)
             logits = self._forward(ctx, ctx.want_rows, bucket)
-            ops.sample(logits, ctx.extra, sampled)
+            if beams is None:
+                ops.sample(logits, ctx.extra, sampled)
+            else:
+                st["chosen"] = self._choose(ctx, beams, logits)
             return logits
 
         if st["graph"] is None:
@@ -383,5 +449,8 @@ class StepRunner:
             # the eager run above already did this step's work; the recorded graph is used from the next step on
         else:
             st["graph"].replay()
-        ctx.sampled = sampled[:S]
+        if beams is None:
+            ctx.sampled = sampled[:S]
+        else:
+            ctx.chosen = tuple(t[:S // unit] for t in st["chosen"])
         return st["logits"][:S], ctx

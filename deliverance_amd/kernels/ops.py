@@ -356,7 +356,7 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
     any numbers 0 .. B - 1, in any order and with repeats.  ``slots`` and ``parents``: int32 [G, B] on the device, the slots distinct;
     a place whose slot is no row (negative, say) or whose parent is outside 0 .. B - 1 is left as it is.
     The rows lie along dimension ``dim``: tensors [rows, ...], or, with 1, [layers, rows, ...].  They must be contiguous, have equally
-    many rows of whole 4-byte words, and share no memory."""
+    many rows of whole 2-byte units, and share no memory."""
     _dev_here(slots, parents, *tensors)
     _need(slots.dtype == parents.dtype == torch.int32 and slots.dim() == 2 and slots.shape == parents.shape and slots.is_contiguous()
           and parents.is_contiguous(), "state_reorder: slots and parents must be contiguous int32 [groups, places]")
@@ -374,8 +374,8 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
         size = t.numel() * t.element_size()
         ptrs[i], layers[i] = _ptr(t), t.shape[0] if dim else 1
         row_bytes[i] = size // max(1, pool * layers[i])
-        if size and (row_bytes[i] == 0 or row_bytes[i] % 4):
-            raise KernelError(f"state_reorder: a row of tensor {i} has {row_bytes[i]} bytes, whole 4-byte words are needed")
+        if row_bytes[i] % 2:
+            raise KernelError(f"state_reorder: a row of tensor {i} has {row_bytes[i]} bytes, whole 2-byte units are needed")
         if size == 0:
             layers[i], row_bytes[i] = 0, 4
         spans.append((t.data_ptr(), size))
@@ -1400,11 +1400,17 @@ def attention_both(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torch
     return out
 
 
+def attention_beams_pays(ctx, group: int, n_heads: int, n_kv_heads: int, head_dim: int, page: int) -> bool:
+    """Whether a step's attention goes to ``attention_beams``: a step of beams, sizes that it takes, the tuned kernels."""
+    return _MODE == "tuned" and ctx.n_beams > 1 and ctx.n_decode == ctx.n_seqs and attention_beams_takes(head_dim, page)
+
+
 def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, n_heads: int,
                     scale: float, window: Optional[int], out: torch.Tensor) -> torch.Tensor:
     """Attention of every row of the step over its sequence's pages.  In bfloat16 the one-token
     sequences (the first ``ctx.n_decode``) go to the decode kernel and the portions to the
-    prefill kernel, in 32-bit both to one kernel; the reference mode and head sizes that are no multiple of 16
+    prefill kernel, in 32-bit both to one kernel; the beams of a search, whose tables begin with the same pages, to the kernel
+    that reads those once, where that pays; the reference mode and head sizes that are no multiple of 16
     (which the matrix-core kernels do not take) use the plain kernel for all rows."""
     bt = ctx.block_tables[group]
     Hkv, page, D = cache_slot.shape[2], cache_slot.shape[3], cache_slot.shape[4]
@@ -1427,6 +1433,11 @@ def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, 
             pairs += sum(min(n - t + i + 1, window or n) for i in range(t)) if t > 1 else min(n, window or n)
         return keys * 2 * Hkv * D * el + 2 * rows * n_heads * D * el, 4 * pairs * n_heads * D
 
+    if ctx.n_beams > 1 and attention_beams_pays(ctx, group, n_heads, Hkv, D, page) and q.stride(0) * el % 16 == 0 and q.data_ptr() % 16 == 0:
+        n_splits = beam_splits(nd // ctx.n_beams, ctx.n_beams, n_heads, Hkv, D, bt.shape[1], page)
+        ws = ctx.flat("beam_partial", beam_workspace_floats(nd, n_heads, D, n_splits), torch.float32) if n_splits > 1 else None
+        with _timed("attention_beams", *cost(0, nd), "fp32" if el == 4 else "bf16"):
+            return attention_beams(q, cache_slot, bt, ctx.seq_lens, ctx.beam_shared[group], ctx.n_beams, n_heads, scale, window, out, n_splits, ws)
     if _MODE == "tuned" and q.dtype == torch.bfloat16 and D % 16 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
         n_splits = decode_splits(nd, n_heads, bt.shape[1], page) if nd else 1
         if nd and _lib().da_attn_both_pays(nd, ctx.n_seqs - nd, ctx.max_query_len, n_heads, D, page, n_splits, bt.shape[1]):

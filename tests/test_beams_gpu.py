@@ -172,7 +172,7 @@ def test_rows_follow_their_parents(groups, beams, row):
     g = torch.Generator().manual_seed(groups * 100 + beams + row)
     pool = groups * beams + 3
     tensors = [torch.randint(-2 ** 31, 2 ** 31 - 1, (pool, row), generator=g, dtype=torch.int32).to(DEV),       # any bits, also of no numbers
-               torch.randn(pool, 2, row, generator=g).to(torch.bfloat16).to(DEV)]
+               torch.randn(pool, row, generator=g).to(torch.bfloat16).to(DEV)]
     for kind in ("any", "permutation", "one", "none"):
         slots = torch.randperm(pool, generator=g)[:groups * beams].view(groups, beams).int()
         if kind == "any":
@@ -209,7 +209,7 @@ def test_refusals_of_reordering():
     ops.state_reorder([torch.zeros(6, 0, device=DEV)], i, i)
     wide = torch.zeros(1, 65, dtype=torch.int32, device=DEV)
     for args in (([t], i.long(), i.long()), ([t], i, i[:1]), ([t], i.view(-1), i.view(-1)), ([t.t()], i, i), ([t, t[:5]], i, i), ([t, t], i, i),
-                 ([t, t.view(-1)[4:].view(5, 4)], i, i), ([torch.zeros(6, 3, dtype=torch.bfloat16, device=DEV)], i, i), ([t], i, i, 2),
+                 ([t, t.view(-1)[4:].view(5, 4)], i, i), ([torch.zeros(6, 3, dtype=torch.uint8, device=DEV)], i, i), ([t], i, i, 2),
                  ([t], wide, wide), ([t], i.t(), i.t())):
         with pytest.raises(KernelError):
             ops.state_reorder(*args)
