@@ -17,6 +17,7 @@
 // bfloat16: a 32-bit weight goes in as two bfloat16 parts (16 bits; one part alone would lose as much again as the result's own
 // rounding).  32-bit: 16x16x4 products, nothing is rounded.
 #include "gemm_common.h"
+#include <da_lane_swap.h>
 
 #define BEAMS_MAX 64             // beams of a group
 #define BEAMS_MAX_D 256
@@ -24,20 +25,42 @@
 #define ROWS 16                  // of a workgroup
 #define BEAM_WAVES 4
 
-__device__ __forceinline__ float beam_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+struct Yes { static const bool value = true; };
+struct No { static const bool value = false; };
 
-// Row maximum over the four lanes that hold a row's keys
+// 2^x: scores carry log2 e in their scale
+__device__ __forceinline__ float exp_of_2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Over the four lanes that hold a row's keys
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, DA_WAVE));
-  return fmaxf(v, __shfl_xor(v, 32, DA_WAVE));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor(v, 16, DA_WAVE);
-  return v + __shfl_xor(v, 32, DA_WAVE);
+  return half_max(v);
 }
 
-// DK: head size in steps of 32, rounded up to a power of two
-template <typename T, int DK>
+// Over the wavefront, in every lane
+template <class Op>
+__device__ __forceinline__ int wave_join(int v, Op op) {
+  v = op(v, dpp_move_i<0xB1, 0xF>(v, v));
+  v = op(v, dpp_move_i<0x4E, 0xF>(v, v));
+  v = op(v, dpp_move_i<0x141, 0xF>(v, v));
+  v = op(v, dpp_move_i<0x140, 0xF>(v, v));
+  v = op(v, dpp_move_i<0x142, 0xA>(v, v));
+  v = op(v, dpp_move_i<0x143, 0xC>(v, v));
+  return __builtin_amdgcn_readlane(v, DA_WAVE - 1);
+}
+// the sum of the lanes up to this one
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_move_i<0x111, 0xF>(0, v);
+  v += dpp_move_i<0x112, 0xF>(0, v);
+  v += dpp_move_i<0x114, 0xF>(0, v);
+  v += dpp_move_i<0x118, 0xF>(0, v);
+  v += dpp_move_i<0x142, 0xA>(0, v);
+  v += dpp_move_i<0x143, 0xC>(0, v);
+  return v;
+}
+
+// DK: head size in steps of 32, rounded up to a power of two.  STEP: keys whose loads are under way together.
+template <typename T, int DK, int STEP>
 __global__ void __launch_bounds__(BEAM_WAVES * DA_WAVE)
 attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache, const int* __restrict__ block_table, int max_blocks,
                   const int* __restrict__ seq_lens, const int* __restrict__ shared, int B, int Hq, int Hkv, int D, int page, float scale,
@@ -45,56 +68,25 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int DV = 2 * DK, DMAX = 32 * DK;            // value dimensions in steps of 16
   constexpr int QS = F32 ? 2 * DK : DK;                 // key loads a row: 16 dimensions (32-bit) or 32 (bfloat16) a step
+  constexpr int KP = STEP / 16;                         // pieces of 16 keys
+  constexpr int VP = F32 ? STEP / 16 : STEP / 32;       // value loads a dimension: 4 keys (32-bit) or 8 a lane
+  constexpr int SPAN = F32 ? 4 : 8;                     // consecutive keys of a lane
   __shared__ float acc_lds[BEAM_WAVES][DMAX][ROWS + 1];
   __shared__ float m_lds[BEAM_WAVES][ROWS], l_lds[BEAM_WAVES][ROWS];
-  __shared__ int len_lds[BEAMS_MAX];
 
   const int t = threadIdx.x, lane = t % DA_WAVE, wave = __builtin_amdgcn_readfirstlane(t / DA_WAVE);
   const int col = lane % 16, quad = lane / 16;
   const int ratio = Hq / Hkv, R = B * ratio;
   const int hk = blockIdx.x % Hkv, rb = blockIdx.x / Hkv, g = blockIdx.y, z = blockIdx.z;
-  const int r0 = rb * ROWS, r_last = min(r0 + ROWS, R) - 1;
-  const int b0 = r0 / ratio, b1 = r_last / ratio;       // the beams of these rows
-  const int s0 = g * B;
+  const int r0 = rb * ROWS, s0 = g * B;
+  const int b0 = r0 / ratio, b1 = (min(r0 + ROWS, R) - 1) / ratio;      // the beams of these rows
   const int lg = 31 - __builtin_clz(page), pmask = page - 1;
   const uint32_t page_elems = 2u * (uint32_t)(Hkv * page * D);
-
-  // this lane's row
-  const int r = r0 + col, beam = min(r, R - 1) / ratio, head = hk * ratio + (min(r, R - 1) - beam * ratio);
   const int cap = max_blocks * page;                    // (a longer length would lead out of the table)
-  const int len = r < R ? min(seq_lens[s0 + beam], cap) : 0;
-  const int lo = window > 0 && len - window > 0 ? len - window : 0;
 
-  // the positions that every beam of the group has in shared pages, and from which on every row of this workgroup sees them
-  int first_live = -1, common = cap, lo_max = 0;
-  for (int b = 0; b < B; ++b) {
-    const int n = min(seq_lens[s0 + b], cap);
-    if (n <= 0) continue;
-    if (first_live < 0) first_live = b;
-    common = min(common, n);
-    if (window > 0 && n - window > lo_max) lo_max = n - window;
-  }
-  common = first_live < 0 ? 0 : min(common, shared[g]);
-  const int shared0 = (lo_max + CHUNK - 1) / CHUNK, shared1 = common / CHUNK > shared0 ? common / CHUNK : shared0;
-  auto own_chunks = [&](int b, int& first, int& skip_at, int& skip_to) {      // number of the beam's own chunks
-    const int n = min(seq_lens[s0 + b], cap);
-    if (n <= 0) return 0;
-    first = window > 0 && n - window > 0 ? (n - window) / CHUNK : 0;
-    const int end = (n + CHUNK - 1) / CHUNK;
-    skip_at = shared0;
-    skip_to = shared1;
-    // chunks first .. end - 1 without shared0 .. shared1 - 1
-    return end - first - (shared1 - shared0);
-  };
-  int items = shared1 - shared0;
-  for (int b = b0; b <= b1; ++b) {
-    int f, a, e;
-    items += own_chunks(b, f, a, e);
-  }
-  const int per = (items + splits - 1) / splits;
-  const int item0 = z * per, item1 = min(items, item0 + per);
-
-  // the query rows: the right operand
+  // a beam a lane: its length; then the query rows, the right operand (row r of the group is column r - r0)
+  const int n_raw = seq_lens[s0 + (lane < B ? lane : 0)], shared_g = shared[g];
+  const int r = r0 + col, rr = min(r, R - 1), beam = rr / ratio, head = hk * ratio + (rr - beam * ratio);
   uint4 qf[QS];
 #pragma unroll
   for (int k = 0; k < QS; ++k) {
@@ -102,110 +94,148 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
     qf[k] = make_uint4(0, 0, 0, 0);
     if (d < D && r < R) qf[k] = *(const uint4*)(q + (size_t)(s0 + beam) * q_ld + (size_t)head * D + d);
   }
+  const int n_b = lane < B ? max(0, min(n_raw, cap)) : 0, lo_b = window > 0 ? max(0, n_b - window) : 0;
+  const uint64_t alive = __builtin_amdgcn_ballot_w64(n_b > 0);
+  const int first_live = alive ? __builtin_ctzll(alive) : 0;
+  // shared chunks: those that all beams have in shared pages, and all see from their first position on
+  const int common = min(shared_g, wave_join(n_b > 0 ? n_b : 0x7fffffff, [](int a, int b) { return min(a, b); }));
+  const int shared0 = alive ? (wave_join(lo_b, [](int a, int b) { return max(a, b); }) + CHUNK - 1) / CHUNK : 0;
+  const int shared1 = alive ? max(shared0, common / CHUNK) : 0;
+  // a beam's own chunks: from its first one on to its last, without the shared ones
+  const int own0 = lo_b / CHUNK, own = lane >= b0 && lane <= b1 && n_b > 0 ? (n_b + CHUNK - 1) / CHUNK - own0 - (shared1 - shared0) : 0;
+  const int own_to = wave_scan(own);
+  const int n_shared = shared1 - shared0, items = n_shared + __builtin_amdgcn_readlane(own_to, DA_WAVE - 1);
+  const int per = (items + splits - 1) / splits;
+  const int item0 = z * per, item1 = min(items, item0 + per);
+  const int len_of_beam = __shfl(n_b, beam, DA_WAVE), lo = __shfl(lo_b, beam, DA_WAVE), len = r < R ? len_of_beam : 0;
+  const float scale2 = scale * 1.4426950408889634f;
 
   floatx4 acc[DV];
 #pragma unroll
   for (int i = 0; i < DV; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+  const T* const kbase = cache + (size_t)hk * page * D;
+  const T* const vbase = cache + (size_t)(Hkv + hk) * page * D;
 
   for (int item = item0 + wave; item < item1; item += BEAM_WAVES) {
-    // which chunk of which table
-    int chunk, mine = -1, src = first_live;
-    if (item < shared1 - shared0) chunk = shared0 + item;
-    else {
-      int left = item - (shared1 - shared0), f = 0, a = 0, e = 0;
-      for (mine = b0; mine < b1; ++mine) {
-        const int n = own_chunks(mine, f, a, e);
-        if (left < n) break;
-        left -= n;
-      }
-      own_chunks(mine, f, a, e);
-      chunk = f + left;
-      if (e > a && chunk >= a) chunk += e - a;
+    // which chunk of whose table (own < 0: of all)
+    int chunk = shared0 + item, mine = -1, src = first_live, first = 0, last = 0x7fffffff;
+    if (item >= n_shared) {
+      const int left = item - n_shared;
+      mine = __builtin_popcountll(__builtin_amdgcn_ballot_w64(own_to <= left));
+      mine = min(mine, b1);
+      chunk = __builtin_amdgcn_readlane(own0, mine) + left - (__builtin_amdgcn_readlane(own_to, mine) - __builtin_amdgcn_readlane(own, mine));
+      if (chunk >= shared0) chunk += n_shared;
       src = mine;
+      first = max(chunk * CHUNK, __builtin_amdgcn_readlane(lo_b, mine));
+      last = min(chunk * CHUNK + CHUNK, __builtin_amdgcn_readlane(n_b, mine)) - 1;
+    } else {
+      first = chunk * CHUNK;
+      last = first + CHUNK - 1;
     }
     const int* bt = block_table + (size_t)(s0 + src) * max_blocks;
-    const int n_src = min(seq_lens[s0 + src], cap), lo_src = window > 0 && n_src - window > 0 ? n_src - window : 0;
-    const int c0 = chunk * CHUNK;
-    const int first = mine < 0 ? c0 : max(c0, lo_src), last = mine < 0 ? c0 + CHUNK - 1 : min(c0 + CHUNK, n_src) - 1;
     const bool takes = mine < 0 || mine == beam;
 
-#pragma unroll 1
-    for (int h0 = c0; h0 < c0 + CHUNK; h0 += 32) {      // 32 keys at a time
-      if (h0 > last || h0 + 31 < first) continue;
-      floatx4 sc[2];
+    auto step = [&](int h0, auto cut_tag) {
+      constexpr bool CUT = decltype(cut_tag)::value;
+      // ---- every load of the step, then the arithmetic.  A lane's keys of the first product lie in one group of 8 (bfloat16), or are one
+      // key a piece; keys and values that nobody sees are read from a place that somebody does.
+      uint4 kf[KP][QS], vf[VP][DV];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-        const int key = h0 + (F32 ? 16 * j + col : 8 * (col / 4) + 4 * j + col % 4);
-        const int seen = key < first ? first : (key > last ? last : key);
-        const int pg = max(bt[seen >> lg], 0);
-        const T* kp = cache + (size_t)pg * page_elems + ((size_t)hk * page + (seen & pmask)) * D;
+      for (int j = 0; j < KP; ++j) {
+        const int key = h0 + (F32 ? 16 * j + col : 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4);
+        const int seen = CUT ? max(first, min(last, key)) : key;
+        const T* kp = kbase + (size_t)(uint32_t)max(bt[seen >> lg], 0) * page_elems + (size_t)(seen & pmask) * D;
 #pragma unroll
         for (int k = 0; k < QS; ++k) {
           const int d = F32 ? 16 * k + 4 * quad : 32 * k + 8 * quad;
-          uint4 kf = make_uint4(0, 0, 0, 0);
-          if (d < D) kf = *(const uint4*)(kp + d);
+          // (a step that can lie past D: zeros, not a neighbour's numbers, of which zero times an infinite one is no number)
+          if (2 * k + 2 <= QS && QS > 1) kf[j][k] = *(const uint4*)(kp + d);
+          else {
+            kf[j][k] = make_uint4(0, 0, 0, 0);
+            if (d < D) kf[j][k] = *(const uint4*)(kp + d);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VP; ++j) {
+        const int k0 = h0 + 4 * SPAN * j + SPAN * quad;  // the lane's first key
+        const bool any = !CUT || (k0 <= last && k0 + SPAN - 1 >= first);
+        const int at = any ? k0 : (first & ~(SPAN - 1));
+        const T* vp = vbase + (size_t)(uint32_t)max(bt[at >> lg], 0) * page_elems + (size_t)col * page + (at & pmask);
+#pragma unroll
+        for (int i = 0; i < DV; ++i) {
+          vf[j][i] = *(const uint4*)vp;
+          vp += 16 * (i + 1) < D ? 16 * page : 0;        // (a piece past D reads the last one again and is dropped)
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      floatx4 sc[KP];
+#pragma unroll
+      for (int j = 0; j < KP; ++j) sc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < QS; ++k)
+#pragma unroll
+        for (int j = 0; j < KP; ++j) {
           if (F32) {
-            const uint32_t ka[4] = {kf.x, kf.y, kf.z, kf.w}, qa[4] = {qf[k].x, qf[k].y, qf[k].z, qf[k].w};
+            const uint32_t ka[4] = {kf[j][k].x, kf[j][k].y, kf[j][k].z, kf[j][k].w}, qa[4] = {qf[k].x, qf[k].y, qf[k].z, qf[k].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka[i]), __uint_as_float(qa[i]), sc[j], 0, 0, 0);
           } else {
-            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[k]), sc[j], 0, 0, 0);
+            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[j][k]), __builtin_bit_cast(bf16x8_t, qf[k]), sc[j], 0, 0, 0);
           }
         }
-      }
-      // this lane's 8 keys: key_of(j, i)
-      float s[2][4], top = -INFINITY;
+      // ---- the lane's keys: four a piece, of column col's row
+      float e[KP][4], top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < KP; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = h0 + (F32 ? 16 * j + 4 * quad + i : 8 * quad + 4 * j + i);
-          const bool sees = takes && key >= first && key <= last && key >= lo && key < len;
-          s[j][i] = sees ? sc[j][i] * scale : -INFINITY;
-          top = fmaxf(top, s[j][i]);
+          e[j][i] = sc[j][i] * scale2;
+          if (CUT) {
+            const int key = h0 + (F32 ? 16 * j + 4 * quad + i : 32 * (j / 2) + 8 * quad + 4 * (j % 2) + i);
+            e[j][i] = takes && key >= lo && key < len ? e[j][i] : -INFINITY;
+          }
+          top = fmaxf(top, e[j][i]);
         }
       const float m_new = fmaxf(m, quad_max(top)), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = beam_exp(m - m_use);
+      const float alpha = exp_of_2(m - m_use);
       m = m_new;
-      l *= alpha;
-      float e[2][4];
+      float add = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < KP; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[j][i] = beam_exp(s[j][i] - m_use);
-          l += e[j][i];
+          e[j][i] = exp_of_2(e[j][i] - m_use);
+          add += e[j][i];
         }
-      uint4 hi = make_uint4(0, 0, 0, 0), lw = hi;       // bfloat16: the weights' two parts
+      l = l * alpha + add;
+      uint4 hi[VP], lw[VP];                             // bfloat16: the weights' two parts
       if (!F32) {
-        uint32_t h4[4], l4[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float x = e[w / 2][2 * (w % 2)], y = e[w / 2][2 * (w % 2) + 1];
-          h4[w] = pack2_bf16(x, y);
-          l4[w] = pack2_bf16(x - __uint_as_float(h4[w] << 16), y - __uint_as_float(h4[w] & 0xffff0000u));
+        for (int j = 0; j < VP; ++j) {
+          uint32_t h4[4], l4[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float x = e[2 * j + w / 2][2 * (w % 2)], y = e[2 * j + w / 2][2 * (w % 2) + 1];
+            h4[w] = pack2_bf16(x, y);
+            l4[w] = pack2_bf16(x - __uint_as_float(h4[w] << 16), y - __uint_as_float(h4[w] & 0xffff0000u));
+          }
+          hi[j] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+          lw[j] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
         }
-        hi = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-        lw = make_uint4(l4[0], l4[1], l4[2], l4[3]);
       }
-      const bool cut = h0 < first || h0 + 31 > last;
 #pragma unroll
-      for (int j = 0; j < (F32 ? 2 : 1); ++j) {
-        const int k0 = h0 + (F32 ? 16 * j + 4 * quad : 8 * quad), span = F32 ? 4 : 8;      // the lane's keys of the left operand
-        const bool any = k0 <= last && k0 + span - 1 >= first;
-        const int at = any ? k0 : (first & ~(span - 1));
-        const int pg = max(bt[at >> lg], 0);
-        const T* vp = cache + (size_t)pg * page_elems + (size_t)(Hkv + hk) * page * D + (at & pmask);
+      for (int i = 0; i < DV; ++i) {
+        floatx4 o;
 #pragma unroll
-        for (int i = 0; i < DV; ++i) {
-          const int d = 16 * i + col;
-          uint4 vf = make_uint4(0, 0, 0, 0);
-          if (16 * i < D) vf = *(const uint4*)(vp + (size_t)d * page);
-          if (cut) {                                    // rows that are not seen may hold anything
-            uint32_t v4[4] = {vf.x, vf.y, vf.z, vf.w};
+        for (int x = 0; x < 4; ++x) o[x] = acc[i][x] * alpha;
+#pragma unroll
+        for (int j = 0; j < VP; ++j) {
+          uint32_t v4[4] = {vf[j][i].x, vf[j][i].y, vf[j][i].z, vf[j][i].w};
+          if (CUT) {                                    // positions that are not seen may hold anything
+            const int k0 = h0 + 4 * SPAN * j + SPAN * quad;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               if (F32) v4[w] = (k0 + w >= first && k0 + w <= last) ? v4[w] : 0u;
@@ -214,56 +244,61 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
                 v4[w] &= ((ka >= first && ka <= last) ? 0x0000ffffu : 0u) | ((ka + 1 >= first && ka + 1 <= last) ? 0xffff0000u : 0u);
               }
             }
-            vf = make_uint4(v4[0], v4[1], v4[2], v4[3]);
           }
-          if (F32 ? j == 0 : true) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[i][x] *= alpha;
-          }
-          floatx4 o = acc[i];
           if (F32) {
-            const uint32_t v4[4] = {vf.x, vf.y, vf.z, vf.w};
 #pragma unroll
             for (int x = 0; x < 4; ++x) o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v4[x]), e[j][x], o, 0, 0, 0);
           } else {
-            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, hi), o, 0, 0, 0);
-            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, lw), o, 0, 0, 0);
+            const uint4 v = make_uint4(v4[0], v4[1], v4[2], v4[3]);
+            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, hi[j]), o, 0, 0, 0);
+            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, lw[j]), o, 0, 0, 0);
           }
-          // (a column that takes no part keeps its sums: zero times another beam's infinite value is no number)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[i][x] = takes ? o[x] : acc[i][x];
         }
+        // (a column that takes no part keeps its sums: zero times another beam's infinite value is no number)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][x] = !CUT || takes ? o[x] : acc[i][x];
       }
+    };
+    if (mine < 0) {
+#pragma unroll 1
+      for (int h0 = first; h0 <= last; h0 += STEP) step(h0, No{});
+    } else {
+#pragma unroll 1
+      for (int h0 = chunk * CHUNK + (first % CHUNK) / STEP * STEP; h0 <= last; h0 += STEP) step(h0, Yes{});
     }
   }
 
   // ---- the wavefronts' results joined
-  l = quad_sum(l);
+  l += __shfl_xor(l, 16, DA_WAVE);
+  l += __shfl_xor(l, 32, DA_WAVE);
+  if (len <= 0) l = 0.f;                                // (a place without a beam went along in the shared chunks)
   if (quad == 0) {
-    m_lds[wave][col] = m;
+    m_lds[wave][col] = len > 0 ? m : -INFINITY;
     l_lds[wave][col] = l;
   }
 #pragma unroll
   for (int i = 0; i < DV; ++i)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) acc_lds[wave][16 * i + 4 * quad + x][col] = acc[i][x];
+    for (int x = 0; x < 4; ++x) acc_lds[wave][16 * i + 4 * quad + x][col] = len > 0 ? acc[i][x] : 0.f;
   __syncthreads();
   for (int i = t; i < ROWS * D; i += BEAM_WAVES * DA_WAVE) {
     const int row = i / D, d = i - row * D;
     if (r0 + row >= R) break;
     float mm = -INFINITY;
+#pragma unroll
     for (int w = 0; w < BEAM_WAVES; ++w) mm = fmaxf(mm, m_lds[w][row]);
     const float m_use = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f, o = 0.f;
+#pragma unroll
     for (int w = 0; w < BEAM_WAVES; ++w) {
-      const float a = beam_exp(m_lds[w][row] - m_use);
+      const float a = exp_of_2(m_lds[w][row] - m_use);
       ll += a * l_lds[w][row];
       o += a * acc_lds[w][d][row];
     }
     const int bm = (r0 + row) / ratio, hd = hk * ratio + (r0 + row - bm * ratio);
     if (splits == 1) from_f32(out + (size_t)(s0 + bm) * out_ld + (size_t)hd * D + d, ll > 0.f || ll != ll ? o / ll : 0.f);
     else {
-      float* p = partial + ((((size_t)(s0 + bm) * Hq + hd) * splits) + z) * (D + 2);
+      float* p = partial + (((size_t)(s0 + bm) * Hq + hd) * splits + z) * (D + 2);
       p[d] = o;
       if (d == 0) {
         p[D] = mm;
@@ -273,23 +308,32 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   }
 }
 
+// A wavefront a (sequence, head): a share a lane for the maxima and sums, then a dimension a lane.
+#define MERGE_WAVES 4
 template <typename T>
-__global__ void __launch_bounds__(BEAMS_MAX_D)
-attn_beams_merge_kernel(const float* __restrict__ partial, int splits, int Hq, int D, T* __restrict__ out, int out_ld) {
-  const int h = blockIdx.x, s = blockIdx.y, d = threadIdx.x;
-  if (d >= D) return;
-  const float* p = partial + ((size_t)s * Hq + h) * splits * (D + 2);
-  float mm = -INFINITY;
-  for (int z = 0; z < splits; ++z) mm = fmaxf(mm, p[(size_t)z * (D + 2) + D]);
-  const float m_use = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, o = 0.f;
-  for (int z = 0; z < splits; ++z) {
-    const float* pz = p + (size_t)z * (D + 2);
-    const float a = beam_exp(pz[D] - m_use);
-    ll += a * pz[D + 1];
-    o += a * pz[d];
+__global__ void __launch_bounds__(MERGE_WAVES * DA_WAVE)
+attn_beams_merge_kernel(const float* __restrict__ partial, int splits, int pairs, int Hq, int D, T* __restrict__ out, int out_ld) {
+  const int lane = threadIdx.x % DA_WAVE, pair = blockIdx.x * MERGE_WAVES + threadIdx.x / DA_WAVE;
+  if (pair >= pairs) return;
+  const int s = pair / Hq, h = pair - s * Hq;
+  const float* p = partial + (size_t)pair * splits * (D + 2);
+  const float* mine = p + (size_t)(lane < splits ? lane : 0) * (D + 2) + D;
+  const float m = lane < splits ? mine[0] : -INFINITY, l = lane < splits ? mine[1] : 0.f;
+  const float mm = wave_max(m), m_use = mm == -INFINITY ? 0.f : mm;
+  const float w = lane < splits ? exp_of_2(m - m_use) : 0.f;
+  const float ll = wave_sum(w * l), inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+  for (int d0 = 0; d0 < D; d0 += DA_WAVE) {
+    const int d = d0 + lane;
+    float o = 0.f;
+    for (int z0 = 0; z0 < splits; z0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = p[(size_t)min(z0 + u, splits - 1) * (D + 2) + (d < D ? d : 0)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) o += (z0 + u < splits ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(z0 + u, DA_WAVE - 1))) : 0.f) * v[u];
+    }
+    if (d < D) from_f32(out + (size_t)s * out_ld + (size_t)h * D + d, o * inv);
   }
-  from_f32(out + (size_t)s * out_ld + (size_t)h * D + d, ll > 0.f || ll != ll ? o / ll : 0.f);
 }
 
 extern "C" int da_attn_beams_takes(int D, int page) {
@@ -306,12 +350,12 @@ extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int ma
   return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
 }
 
-template <typename T, int DK>
+template <typename T, int DK, int STEP>
 static void beams_launch(hipStream_t s, const void* q, int q_ld, const void* cache, const int* block_table, int max_blocks, const int* seq_lens,
                          const int* shared, int G, int B, int Hq, int Hkv, int D, int page, float scale, int window, void* out, int out_ld,
                          int splits, float* partial) {
   const int blocks = da_ceil_div((long)B * (Hq / Hkv), ROWS);
-  hipLaunchKernelGGL((attn_beams_kernel<T, DK>), dim3(Hkv * blocks, G, splits), dim3(BEAM_WAVES * DA_WAVE), 0, s, (const T*)q, q_ld,
+  hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP>), dim3(Hkv * blocks, G, splits), dim3(BEAM_WAVES * DA_WAVE), 0, s, (const T*)q, q_ld,
                      (const T*)cache, block_table, max_blocks, seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits,
                      partial);
 }
@@ -326,31 +370,30 @@ extern "C" int da_attn_beams(const void* q, int q_ld, const void* cache, int dty
   const int el = dtype == DA_F32 ? 4 : 2;
   DA_REQUIRE((uintptr_t)q % 16 == 0 && (long)q_ld * el % 16 == 0 && (uintptr_t)cache % 16 == 0, "attention_beams: q and the cache must lie on 16 bytes");
   DA_REQUIRE((long)max_blocks * page <= 0x7fffff00L && 2L * Hkv * page * D <= 0x7fffffffL, "attention_beams: a page or a table is too large");
-  DA_REQUIRE(splits >= 1 && splits <= 65535, "attention_beams: %d shares", splits);
+  DA_REQUIRE(splits >= 1 && splits <= DA_WAVE, "attention_beams: %d shares (1 to 64)", splits);
   const long need = splits > 1 ? (long)G * B * Hq * splits * (D + 2) : 0;
   DA_REQUIRE(need == 0 || (workspace && workspace_floats >= need), "attention_beams: %ld floats of workspace are needed, found %ld", need, workspace_floats);
   if (G == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
-#define DA_BEAMS(T, DK) beams_launch<T, DK>(s, q, q_ld, cache, block_table, max_blocks, seq_lens, shared, G, B, Hq, Hkv, D, page, scale, window, out, out_ld, splits, workspace)
+#define DA_BEAMS(T, DK, STEP) beams_launch<T, DK, STEP>(s, q, q_ld, cache, block_table, max_blocks, seq_lens, shared, G, B, Hq, Hkv, D, page, scale, window, out, out_ld, splits, workspace)
   if (dtype == DA_F32) {
-    if (D <= 32) DA_BEAMS(float, 1);
-    else if (D <= 64) DA_BEAMS(float, 2);
-    else if (D <= 128) DA_BEAMS(float, 4);
-    else DA_BEAMS(float, 8);
+    if (D <= 32) DA_BEAMS(float, 1, 32);
+    else if (D <= 64) DA_BEAMS(float, 2, 32);
+    else if (D <= 128) DA_BEAMS(float, 4, 32);
+    else DA_BEAMS(float, 8, 16);
   } else {
-    if (D <= 32) DA_BEAMS(bf16_t, 1);
-    else if (D <= 64) DA_BEAMS(bf16_t, 2);
-    else if (D <= 128) DA_BEAMS(bf16_t, 4);
-    else DA_BEAMS(bf16_t, 8);
+    if (D <= 32) DA_BEAMS(bf16_t, 1, 64);
+    else if (D <= 64) DA_BEAMS(bf16_t, 2, 64);
+    else if (D <= 128) DA_BEAMS(bf16_t, 4, 32);
+    else DA_BEAMS(bf16_t, 8, 32);
   }
 #undef DA_BEAMS
   DA_CHECK_LAUNCH("attention_beams");
   if (splits > 1) {
-    const int threads = da_ceil_div(D, DA_WAVE) * DA_WAVE;
-    if (dtype == DA_F32)
-      hipLaunchKernelGGL((attn_beams_merge_kernel<float>), dim3(Hq, G * B), dim3(threads), 0, s, workspace, splits, Hq, D, (float*)out, out_ld);
-    else
-      hipLaunchKernelGGL((attn_beams_merge_kernel<bf16_t>), dim3(Hq, G * B), dim3(threads), 0, s, workspace, splits, Hq, D, (bf16_t*)out, out_ld);
+    const int pairs = G * B * Hq;
+    const dim3 grid(da_ceil_div(pairs, MERGE_WAVES)), block(MERGE_WAVES * DA_WAVE);
+    if (dtype == DA_F32) hipLaunchKernelGGL((attn_beams_merge_kernel<float>), grid, block, 0, s, workspace, splits, pairs, Hq, D, (float*)out, out_ld);
+    else hipLaunchKernelGGL((attn_beams_merge_kernel<bf16_t>), grid, block, 0, s, workspace, splits, pairs, Hq, D, (bf16_t*)out, out_ld);
     DA_CHECK_LAUNCH("attention_beams (merge)");
   }
   return 0;

@@ -16,31 +16,37 @@ struct ReorderTable {
   int units[REORDER_TENSORS];    // of a row, 16, 4 or 2 bytes each
 };
 
-// NB: places that a thread has registers for
-template <typename U, int NB>
+// NB: places that a thread has registers for; UNITS: columns of a thread
+template <typename U, int NB, int UNITS>
 __global__ void __launch_bounds__(REORDER_THREADS)
 reorder_kernel(const ReorderTable table, const int* __restrict__ slots, const int* __restrict__ parents, int B, int pool) {
-  const int units = table.units[blockIdx.y], c = blockIdx.x * REORDER_THREADS + threadIdx.x;
-  if (c >= units) return;
+  // a place a lane: where its row comes from (-1: it stays) and where it is
+  const int lane = threadIdx.x % DA_WAVE, at = (int)blockIdx.z * B + (lane < B ? lane : 0);
+  const int parent = parents[at], slot = slots[at];
+  const int units = table.units[blockIdx.y];
+  int from = __shfl(slot, (unsigned)parent < (unsigned)B ? parent : lane, DA_WAVE);
+  if (lane >= B || parent == lane || (unsigned)parent >= (unsigned)B || (unsigned)slot >= (unsigned)pool || (unsigned)from >= (unsigned)pool || from == slot) from = -1;
+  if (__builtin_amdgcn_ballot_w64(from >= 0) == 0) return;
   U* data = (U*)table.data[blockIdx.y];
-  const int* slot = slots + (size_t)blockIdx.z * B;
-  const int* parent = parents + (size_t)blockIdx.z * B;
-  U v[NB];
-  int to[NB];
+  const int c = blockIdx.x * (REORDER_THREADS * UNITS) + threadIdx.x;
+  U v[NB][UNITS];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    to[b] = -1;
-    if (b >= B) continue;
-    const int p = parent[b], s = slot[b];
-    if (p == b || (unsigned)p >= (unsigned)B || (unsigned)s >= (unsigned)pool) continue;
-    const int from = slot[p];
-    if ((unsigned)from >= (unsigned)pool || from == s) continue;
-    v[b] = data[(size_t)from * units + c];
-    to[b] = s;
+    const int f = __builtin_amdgcn_readlane(from, b);
+    if (f < 0) continue;
+    const U* row = data + (size_t)f * units;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+      if (c + u * REORDER_THREADS < units) v[b][u] = row[c + u * REORDER_THREADS];
   }
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-    if (to[b] >= 0) data[(size_t)to[b] * units + c] = v[b];
+  for (int b = 0; b < NB; ++b) {
+    if (__builtin_amdgcn_readlane(from, b) < 0) continue;
+    U* row = data + (size_t)__builtin_amdgcn_readlane(slot, b) * units;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+      if (c + u * REORDER_THREADS < units) row[c + u * REORDER_THREADS] = v[b][u];
+  }
 }
 
 // n tensors [layers, pool, row]; `data`, `row_bytes` (even) and `layers` are host arrays.
@@ -61,14 +67,17 @@ extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const 
     int count = 0, longest = 0;
     auto launch = [&]() {
       if (!count) return;
-      const dim3 grid(da_ceil_div(longest, REORDER_THREADS), count, G), block(REORDER_THREADS);
       hipStream_t s = (hipStream_t)stream;
-      if (unit == 16 && B <= 4) hipLaunchKernelGGL((reorder_kernel<uint4, 4>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (unit == 16 && B <= 8) hipLaunchKernelGGL((reorder_kernel<uint4, 8>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (unit == 16) hipLaunchKernelGGL((reorder_kernel<uint4, 16>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (unit == 4 && B <= 16) hipLaunchKernelGGL((reorder_kernel<uint32_t, 16>), grid, block, 0, s, table, slots, parents, B, pool);
-      else if (unit == 4) hipLaunchKernelGGL((reorder_kernel<uint32_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
-      else hipLaunchKernelGGL((reorder_kernel<uint16_t, 64>), grid, block, 0, s, table, slots, parents, B, pool);
+      const dim3 block(REORDER_THREADS);
+#define DA_REORDER(U, NB, UNITS) \
+  hipLaunchKernelGGL((reorder_kernel<U, NB, UNITS>), dim3(da_ceil_div(longest, REORDER_THREADS * UNITS), count, G), block, 0, s, table, slots, parents, B, pool)
+      if (unit == 16 && B <= 4) DA_REORDER(uint4, 4, 2);
+      else if (unit == 16 && B <= 8) DA_REORDER(uint4, 8, 2);
+      else if (unit == 16) DA_REORDER(uint4, 16, 1);
+      else if (unit == 4 && B <= 16) DA_REORDER(uint32_t, 16, 2);
+      else if (unit == 4) DA_REORDER(uint32_t, 64, 1);
+      else DA_REORDER(uint16_t, 64, 1);
+#undef DA_REORDER
       count = longest = 0;
     };
     for (int i = 0; i < n; ++i) {
