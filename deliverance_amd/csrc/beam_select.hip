@@ -25,6 +25,7 @@
 #define CHOOSE_THREADS 1024
 #define CHOOSE_WAVES (CHOOSE_THREADS / DA_WAVE)
 #define GROUPS (CHOOSE_THREADS / 4)
+#define HELD 2                   // segments whose keys a thread keeps
 #define LIST 512                 // segments, and entries, that may be looked at one by one
 
 // a 64-bit number that orders like the key; 0 for one that is never chosen
@@ -136,30 +137,39 @@ __device__ void narrow(uint64_t& least, int& last, int keep, Count count) {
   }
 }
 
+// magic: 2^32 / n_segs rounded up (0: divide), for fewer than 65,536 segments
 __global__ void __launch_bounds__(CHOOSE_THREADS)
 beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int K, const float* __restrict__ scores, int n_segs,
                    int n_parts, const float* __restrict__ seg_max, const float* __restrict__ part_max, const double* __restrict__ part_sum,
-                   float* __restrict__ out_score, int* __restrict__ out_parent, int* __restrict__ out_token) {
+                   float* __restrict__ out_score, int* __restrict__ out_parent, int* __restrict__ out_token, uint32_t magic) {
   __shared__ double base[BEAM_MAX], logsum[BEAM_MAX];     // the score (-inf: no beam); the logarithm of the sum
   __shared__ float top[BEAM_MAX];
-  __shared__ uint64_t group_best[GROUPS];
+  __shared__ __attribute__((aligned(16))) uint64_t group_best[GROUPS];
   __shared__ Chosen list[LIST];
   __shared__ int segs[LIST], counts[CHOOSE_WAVES], n_list[2];
   __shared__ uint64_t least_of[1];
-  const int g = blockIdx.x, t = threadIdx.x, wave = t / DA_WAVE, lane = t % DA_WAVE;
+  const int g = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / DA_WAVE), lane = t % DA_WAVE;
   const size_t row0 = (size_t)g * B;
   const int n = B * n_segs;
 
-  // ---- each row's maximum and the logarithm of its sum
+  // ---- asked for together: a thread's first segments, and the partial results of the wavefront's first row
+  const float* sm = seg_max + row0 * n_segs;
+  float zr[HELD];
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) zr[e] = sm[min(t + e * CHOOSE_THREADS, n - 1)];
   for (int b = wave; b < B; b += CHOOSE_WAVES) {
     const float* pm = part_max + (row0 + b) * n_parts;
     const double* ps = part_sum + (row0 + b) * n_parts;
     const float sc = scores[row0 + b];
-    float m = -INFINITY;
-    for (int i = lane; i < n_parts; i += DA_WAVE) m = fmaxf(m, pm[i]);
+    // (a lane past the end takes the last part's maximum again, and no sum)
+    const float p0 = pm[min(lane, n_parts - 1)], p1 = pm[min(lane + DA_WAVE, n_parts - 1)];
+    const double s0 = ps[min(lane, n_parts - 1)], s1 = ps[min(lane + DA_WAVE, n_parts - 1)];
+    float m = fmaxf(p0, p1);
+    for (int i = lane + 2 * DA_WAVE; i < n_parts; i += DA_WAVE) m = fmaxf(m, pm[i]);
     m = wave_max(m);
-    double s = 0.0;
-    for (int i = lane; i < n_parts; i += DA_WAVE) s += ps[i] * (double)expf(pm[i] == m ? 0.f : pm[i] - m);      // (a part without entries has the sum 0)
+    auto weighed = [&](float p, double s) { return s * (double)expf(p == m ? 0.f : p - m); };      // (a part without entries has the sum 0)
+    double s = (lane < n_parts ? weighed(p0, s0) : 0.0) + (lane + DA_WAVE < n_parts ? weighed(p1, s1) : 0.0);
+    for (int i = lane + 2 * DA_WAVE; i < n_parts; i += DA_WAVE) s += weighed(pm[i], ps[i]);
     s = wave_sum_d(m > -INFINITY ? s : 0.0);
     if (lane == 0) {
       top[b] = m;
@@ -183,27 +193,38 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     for (int w = 0; w < CHOOSE_WAVES; ++w) c += counts[w];
     return c;
   };
+  auto row_of = [&](int i) { return magic ? (int)__umulhi((uint32_t)i, magic) : i / n_segs; };
 
   // ---- a key that K entries reach: the K-th best of the largest keys of GROUPS groups of segments
+  uint64_t held[HELD], best = 0;
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    const int i = t + e * CHOOSE_THREADS;
+    held[e] = i < n ? key_of(row_of(i), zr[e]) : 0;
+    best = larger(best, held[e]);
+  }
+  for (int i = t + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) best = larger(best, key_of(row_of(i), sm[i]));
   auto each_seg = [&](auto f) {
-    int b = t / n_segs, s = t - b * n_segs;
-    for (int i = t; i < n; i += CHOOSE_THREADS) {
-      f(key_of(b, seg_max[row0 * n_segs + i]), i);
-      for (s += CHOOSE_THREADS; s >= n_segs; s -= n_segs) ++b;
-    }
+#pragma unroll
+    for (int e = 0; e < HELD; ++e) f(held[e], t + e * CHOOSE_THREADS);      // (one past the end has the key 0)
+    for (int i = t + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) f(key_of(row_of(i), sm[i]), i);
   };
-  uint64_t best = 0;
-  each_seg([&](uint64_t k, int) { best = larger(best, k); });
   best = larger(best, dpp_u64<0xB1>(best));               // 4 lanes
   best = larger(best, dpp_u64<0x4E>(best));
   if (lane % 4 == 0) group_best[t / 4] = best;
   __syncthreads();
-  if (t < GROUPS) {
-    const uint64_t mine = group_best[t];
+  {
+    // the four threads of a group count, a quarter each, the groups in front of it
     int before = 0;
 #pragma unroll 8
-    for (int j = 0; j < GROUPS; ++j) before += group_best[j] > mine || (group_best[j] == mine && j < t);
-    if (before == K - 1 && mine > 1) *least_of = mine;
+    for (int k = 0; k < GROUPS / 4; ++k) {
+      const int j = 4 * k + t % 4;
+      const uint64_t other = group_best[j];
+      before += other > best || (other == best && j < t / 4);
+    }
+    before += dpp_move_i<0xB1, 0xF>(before, before);
+    before += dpp_move_i<0x4E, 0xF>(before, before);
+    if (before == K - 1 && best > 1) *least_of = best;    // (the four write the same)
   }
   __syncthreads();
   uint64_t least = *least_of;
@@ -324,8 +345,10 @@ extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V
   else
     hipLaunchKernelGGL((beam_stats_kernel<SEGS_MANY>), grid, block, 0, (hipStream_t)stream, logits, ldl, V, n_segs, n_parts, seg_max, part_max, part_sum);
   DA_CHECK_LAUNCH("beam_select (sums)");
+  // i * magic / 2^32 is i / n_segs while i < 2^16 and n_segs < 2^16: the product's error, i * (magic * n_segs - 2^32) / n_segs / 2^32, is below i / 2^32
+  const uint32_t magic = (long)B * n_segs < 65536 && n_segs > 1 ? (uint32_t)(((1ull << 32) + n_segs - 1) / n_segs) : 0;
   hipLaunchKernelGGL(beam_choose_kernel, dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts,
-                     seg_max, part_max, part_sum, out_score, out_parent, out_token);
+                     seg_max, part_max, part_sum, out_score, out_parent, out_token, magic);
   DA_CHECK_LAUNCH("beam_select (choice)");
   return 0;
 }

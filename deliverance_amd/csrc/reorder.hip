@@ -5,47 +5,74 @@
 // A thread holds one column of a row for all places of a group: it reads the columns of the rows that move, all of them, and only
 // then writes.  No other thread touches its columns, so parents may be any permutation, with repeats, and no copy is made.
 // Rows that stay are neither read nor written.
+//
+// Bound by memory: every row that moves is read and written once.  Loads and stores go past the caches: 8 x 8 beams' pages of 48
+// layers of 25 heads, 315 MB, take 63.5 us (4.96 TB/s, a large copy 5.13) and 98 with ordinary ones, states of 543 MB 112 and
+// 207; several columns a thread are behind (2: 64.9, 117).
 #include "common.h"
+#include <da_anew.h>
 
 #define REORDER_TENSORS 96       // of a launch (the table is a kernel argument: nothing is uploaded, a recorded launch keeps it)
 #define REORDER_MAX 64           // places of a group
 #define REORDER_THREADS 256
 
+// (The columns travel as structures: of vectors that are only sometimes loaded the compiler makes copies, and waits for each load: 101 us for 63.5.
+// A row may begin on any 4 bytes.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename U> __device__ __forceinline__ U load_past(const U* p) { return __builtin_nontemporal_load(p); }
+template <typename U> __device__ __forceinline__ void store_past(U* p, U v) { __builtin_nontemporal_store(v, p); }
+template <> __device__ __forceinline__ uint4 load_past<uint4>(const uint4* p) {
+  const u32x4 x = __builtin_nontemporal_load((const u32x4*)p);
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+template <> __device__ __forceinline__ void store_past<uint4>(uint4* p, uint4 v) {
+  const u32x4 x = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(x, (u32x4*)p);
+}
+// (a use of what was loaded: the wait for the loads stands here, once, and not in front of every store, where it would wait for the stores too)
+template <typename U> __device__ __forceinline__ void arrived(U& v) { v = (U)da_anew((uint32_t)v); }
+template <> __device__ __forceinline__ void arrived<uint4>(uint4& v) { v.x = da_anew(v.x); }
+// the words behind the last 16 bytes of a row, one a thread
+template <typename U> __device__ __forceinline__ U load_word(const char*) { return U(); }
+template <> __device__ __forceinline__ uint4 load_word<uint4>(const char* p) { return make_uint4(load_past((const uint32_t*)p), 0, 0, 0); }
+template <typename U> __device__ __forceinline__ void store_word(char*, U) {}
+template <> __device__ __forceinline__ void store_word<uint4>(char* p, uint4 v) { store_past((uint32_t*)p, v.x); }
+
 struct ReorderTable {
   void* data[REORDER_TENSORS];
-  int units[REORDER_TENSORS];    // of a row, 16, 4 or 2 bytes each
+  int bytes[REORDER_TENSORS];    // of a row
 };
 
-// NB: places that a thread has registers for; UNITS: columns of a thread
-template <typename U, int NB, int UNITS>
+// NB: places that a thread has registers for
+template <typename U, int NB>
 __global__ void __launch_bounds__(REORDER_THREADS)
 reorder_kernel(const ReorderTable table, const int* __restrict__ slots, const int* __restrict__ parents, int B, int pool) {
+  const int bytes = table.bytes[blockIdx.y], whole = bytes / (int)sizeof(U), units = whole + bytes % (int)sizeof(U) / 4;
+  if (blockIdx.x * REORDER_THREADS >= (unsigned)units) return;
   // a place a lane: where its row comes from (-1: it stays) and where it is
   const int lane = threadIdx.x % DA_WAVE, at = (int)blockIdx.z * B + (lane < B ? lane : 0);
   const int parent = parents[at], slot = slots[at];
-  const int units = table.units[blockIdx.y];
   int from = __shfl(slot, (unsigned)parent < (unsigned)B ? parent : lane, DA_WAVE);
   if (lane >= B || parent == lane || (unsigned)parent >= (unsigned)B || (unsigned)slot >= (unsigned)pool || (unsigned)from >= (unsigned)pool || from == slot) from = -1;
   if (__builtin_amdgcn_ballot_w64(from >= 0) == 0) return;
-  U* data = (U*)table.data[blockIdx.y];
-  const int c = blockIdx.x * (REORDER_THREADS * UNITS) + threadIdx.x;
-  U v[NB][UNITS];
+  const int c = blockIdx.x * REORDER_THREADS + threadIdx.x;
+  const bool in = c < units, word = c >= whole;           // (all lanes stay: each is asked for its place)
+  char* data = (char*)table.data[blockIdx.y] + (word ? (size_t)whole * sizeof(U) + (size_t)(c - whole) * 4 : (size_t)c * sizeof(U));
+  U v[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int f = __builtin_amdgcn_readlane(from, b);
-    if (f < 0) continue;
-    const U* row = data + (size_t)f * units;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u)
-      if (c + u * REORDER_THREADS < units) v[b][u] = row[c + u * REORDER_THREADS];
+    if (f >= 0 && in) v[b] = word ? load_word<U>(data + (size_t)f * bytes) : load_past((const U*)(data + (size_t)f * bytes));
   }
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    if (__builtin_amdgcn_readlane(from, b) < 0) continue;
-    U* row = data + (size_t)__builtin_amdgcn_readlane(slot, b) * units;
+  for (int b = 0; b < NB; ++b) arrived(v[b]);
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u)
-      if (c + u * REORDER_THREADS < units) row[c + u * REORDER_THREADS] = v[b][u];
+  for (int b = 0; b < NB; ++b) {
+    const int f = __builtin_amdgcn_readlane(from, b), to = __builtin_amdgcn_readlane(slot, b);
+    if (f >= 0 && in) {
+      if (word) store_word(data + (size_t)to * bytes, v[b]);
+      else store_past((U*)(data + (size_t)to * bytes), v[b]);
+    }
   }
 }
 
@@ -60,7 +87,7 @@ extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const 
   if (n == 0 || G == 0 || B == 1 || pool == 0) return 0;
   auto unit_of = [&](int i) {
     const uintptr_t odd = (uintptr_t)data[i] | (uintptr_t)row_bytes[i];
-    return B <= 16 && odd % 16 == 0 ? 16 : (odd % 4 == 0 ? 4 : 2);
+    return odd % 4 ? 2 : (B <= 16 ? 16 : 4);
   };
   for (int unit = 16; unit > 1; unit = unit == 16 ? 4 : unit - 2) {      // 16, 4, 2
     ReorderTable table;
@@ -69,14 +96,13 @@ extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const 
       if (!count) return;
       hipStream_t s = (hipStream_t)stream;
       const dim3 block(REORDER_THREADS);
-#define DA_REORDER(U, NB, UNITS) \
-  hipLaunchKernelGGL((reorder_kernel<U, NB, UNITS>), dim3(da_ceil_div(longest, REORDER_THREADS * UNITS), count, G), block, 0, s, table, slots, parents, B, pool)
-      if (unit == 16 && B <= 4) DA_REORDER(uint4, 4, 2);
-      else if (unit == 16 && B <= 8) DA_REORDER(uint4, 8, 2);
-      else if (unit == 16) DA_REORDER(uint4, 16, 1);
-      else if (unit == 4 && B <= 16) DA_REORDER(uint32_t, 16, 2);
-      else if (unit == 4) DA_REORDER(uint32_t, 64, 1);
-      else DA_REORDER(uint16_t, 64, 1);
+#define DA_REORDER(U, NB) \
+  hipLaunchKernelGGL((reorder_kernel<U, NB>), dim3(da_ceil_div(longest, REORDER_THREADS), count, G), block, 0, s, table, slots, parents, B, pool)
+      if (unit == 16 && B <= 4) DA_REORDER(uint4, 4);
+      else if (unit == 16 && B <= 8) DA_REORDER(uint4, 8);
+      else if (unit == 16) DA_REORDER(uint4, 16);
+      else if (unit == 4) DA_REORDER(uint32_t, 64);
+      else DA_REORDER(uint16_t, 64);
 #undef DA_REORDER
       count = longest = 0;
     };
@@ -84,8 +110,9 @@ extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const 
       if (unit_of(i) != unit) continue;
       for (int layer = 0; layer < layers[i]; ++layer) {
         table.data[count] = (char*)data[i] + (long)layer * pool * row_bytes[i];
-        table.units[count] = (int)(row_bytes[i] / unit);
-        longest = table.units[count] > longest ? table.units[count] : longest;
+        table.bytes[count] = (int)row_bytes[i];
+        const int units = (int)(row_bytes[i] / unit) + (unit == 16 ? (int)(row_bytes[i] % 16 / 4) : 0);
+        longest = units > longest ? units : longest;
         if (++count == REORDER_TENSORS) launch();
       }
     }

@@ -326,6 +326,7 @@ class StepRunner:
         per = n // beams.n_beams
         ctx.n_beams = beams.n_beams
         ctx.beam_scores = ctx.extra[:n].view(torch.float32)
+        ctx.beam_shared_host = beams.shared
         ctx.beam_shared = [ctx.extra[n + g * per:n + (g + 1) * per] for g in range(G)]
 
     def _choose(self, ctx, beams: BeamStep, logits: torch.Tensor):

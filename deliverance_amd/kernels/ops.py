@@ -45,7 +45,7 @@ _PINNED_STREAM = None
 def _stream():
     if _PINNED_STREAM is not None:
         return _PINNED_STREAM
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())      # (0.2 us; torch.cuda.current_stream().cuda_stream 2.7)
 
 
 class pinned_stream:
@@ -252,9 +252,13 @@ def _dev(*ts):
 def _dev_here(*ts):
     """``_dev``, and on the device whose current stream the launch goes to."""
     _dev(*ts)
+    here = -1
     for t in ts:
-        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
-            raise KernelError(f"kernel operands lie on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is not None and t.is_cuda:
+            if here < 0:
+                here = torch._C._cuda_getDevice()
+            if t.get_device() != here:
+                raise KernelError(f"kernel operands lie on {t.device}, the current device is cuda:{here}")
 
 
 def _rows_2d(t: torch.Tensor, name: str):
@@ -358,31 +362,37 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
     The rows lie along dimension ``dim``: tensors [rows, ...], or, with 1, [layers, rows, ...].  They must be contiguous, have equally
     many rows of whole 2-byte units, and share no memory."""
     _dev_here(slots, parents, *tensors)
-    _need(slots.dtype == parents.dtype == torch.int32 and slots.dim() == 2 and slots.shape == parents.shape and slots.is_contiguous()
-          and parents.is_contiguous(), "state_reorder: slots and parents must be contiguous int32 [groups, places]")
+    if not (slots.dtype == parents.dtype == torch.int32 and slots.dim() == 2 and slots.shape == parents.shape and slots.is_contiguous()
+            and parents.is_contiguous()):
+        raise KernelError("state_reorder: slots and parents must be contiguous int32 [groups, places]")
     G, B = slots.shape
-    _need(1 <= B <= MAX_BEAMS, f"state_reorder: {B} places a group (1 to {MAX_BEAMS})")
-    _need(dim in (0, 1), "state_reorder: rows along dimension 0 or 1")
+    if not 1 <= B <= MAX_BEAMS or dim not in (0, 1):
+        raise KernelError(f"state_reorder: {B} places a group (1 to {MAX_BEAMS}), rows along dimension {dim} (0 or 1)")
     n = len(tensors)
     if n == 0:
         return tensors
     pool = tensors[0].shape[dim] if tensors[0].dim() > dim else -1
-    ptrs, row_bytes, layers, spans = (ctypes.c_void_p * n)(), (ctypes.c_long * n)(), (ctypes.c_int * n)(), []
+    ptrs, row_bytes, layers, spans = [], [], [], []
     for i, t in enumerate(tensors):
         if t.dim() <= dim or t.shape[dim] != pool or not t.is_contiguous():
             raise KernelError(f"state_reorder: tensor {i} is {list(t.shape)}: contiguous tensors with {pool} rows along dimension {dim} are needed")
-        size = t.numel() * t.element_size()
-        ptrs[i], layers[i] = _ptr(t), t.shape[0] if dim else 1
-        row_bytes[i] = size // max(1, pool * layers[i])
-        if row_bytes[i] % 2:
-            raise KernelError(f"state_reorder: a row of tensor {i} has {row_bytes[i]} bytes, whole 2-byte units are needed")
-        if size == 0:
-            layers[i], row_bytes[i] = 0, 4
+        size, k = t.numel() * t.element_size(), t.shape[0] if dim else 1
+        row = size // (pool * k) if size else 2
+        if row % 2:
+            raise KernelError(f"state_reorder: a row of tensor {i} has {row} bytes, whole 2-byte units are needed")
+        ptrs.append(_ptr(t))
+        row_bytes.append(row)
+        layers.append(k if size else 0)
         spans.append((t.data_ptr(), size))
-    spans.sort()
-    _need(all(a + size <= b for (a, size), (b, _) in zip(spans, spans[1:])), "state_reorder: two tensors share memory")
+    if n > 1:
+        spans.sort()
+        end = 0
+        for a, size in spans:
+            if a < end and size:
+                raise KernelError("state_reorder: two tensors share memory")
+            end = max(end, a + size)
     with _timed("state_reorder", 2 * G * B * sum(r * k for r, k in zip(row_bytes, layers)) if KernelProfiler.enabled else 0, 0, "fp32"):
-        _check(_lib().da_state_reorder(ptrs, row_bytes, layers, n, pool, _ptr(slots), _ptr(parents), G, B, _stream()))
+        _check(_lib().da_state_reorder((ctypes.c_void_p * n)(*ptrs), (ctypes.c_long * n)(*row_bytes), (ctypes.c_int * n)(*layers), n, pool, _ptr(slots), _ptr(parents), G, B, _stream()))
     return tensors
 
 
@@ -857,16 +867,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace)
     _rows_2d(logits, "logits")
     R, V = logits.shape
-    _need(logits.dtype == scores.dtype == torch.float32, "beam_select: logits and scores must be float32")
-    _need(1 <= n_beams <= MAX_BEAMS and R % n_beams == 0, f"beam_select: {R} rows in groups of {n_beams} (1 to {MAX_BEAMS})")
-    G = R // n_beams
-    _need(scores.is_contiguous() and scores.numel() == R, "beam_select: one score a row")
-    K = out_scores.shape[-1]
-    _need(1 <= K <= MAX_CANDIDATES, f"beam_select: {K} candidates (1 to {MAX_CANDIDATES})")
+    if not 1 <= n_beams <= MAX_BEAMS or R % n_beams:
+        raise KernelError(f"beam_select: {R} rows in groups of {n_beams} (1 to {MAX_BEAMS})")
+    if logits.dtype != torch.float32 or scores.dtype != torch.float32 or scores.numel() != R or not scores.is_contiguous():
+        raise KernelError("beam_select: logits and scores must be float32, one score a row")
+    shape = (R // n_beams, out_scores.shape[-1] if out_scores.dim() else 0)
+    if not 1 <= shape[1] <= MAX_CANDIDATES:
+        raise KernelError(f"beam_select: {shape[1]} candidates (1 to {MAX_CANDIDATES})")
     for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32)):
-        if t.dtype != dtype or tuple(t.shape) != (G, K) or not t.is_contiguous():
-            raise KernelError(f"beam_select: outputs must be contiguous [{G}, {K}], float32 scores and int32 parents and tokens")
-    _need(workspace.dtype == torch.float32 and workspace.is_contiguous(), "beam_select: the workspace must be contiguous float32")
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            raise KernelError(f"beam_select: outputs must be contiguous {list(shape)}, float32 scores and int32 parents and tokens")
+    if workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise KernelError("beam_select: the workspace must be contiguous float32")
+    G, K = shape
     with _timed("beam_select", 4 * R * V, 4 * R * V, "fp32"):
         _check(_lib().da_beam_select(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), K, _ptr(out_scores), _ptr(out_parents),
                                      _ptr(out_tokens), _ptr(workspace), workspace.numel(), _stream()))
@@ -1345,15 +1358,21 @@ def attention_beams(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torc
     a group's positions are shared out over that many workgroups, whose partial results pass through ``workspace`` (float32,
     ``beam_workspace_floats`` elements)."""
     _dev_here(q, cache_slot, block_table, seq_lens, shared, out, workspace)
-    Hkv, page, D = _attn_common(q, cache_slot, block_table, n_heads, out, "attention_beams", q.dtype)
+    _rows_2d(q, "q"); _rows_2d(out, "out")
+    if cache_slot.dim() != 5 or cache_slot.shape[1] != 2 or not cache_slot.is_contiguous():
+        raise KernelError("attention_beams: cache slot must be contiguous [pages,2,Hkv,page,D]")
+    _, _, Hkv, page, D = cache_slot.shape
     S = seq_lens.numel()
-    _need(1 <= n_beams <= MAX_BEAMS and S % n_beams == 0, f"attention_beams: {S} sequences in groups of {n_beams} (1 to {MAX_BEAMS})")
-    G = S // n_beams
-    _need(q.shape[0] == S and out.shape[0] == S and block_table.shape[0] >= S, "attention_beams: q, out and block_table must have a row a sequence")
-    _need(seq_lens.dtype == shared.dtype == torch.int32 and seq_lens.is_contiguous() and shared.is_contiguous() and shared.numel() == G,
-          "attention_beams: seq_lens must be int32 [groups * beams], shared int32 [groups]")
-    _need(n_splits <= 1 or (workspace is not None and workspace.dtype == torch.float32 and workspace.is_contiguous()),
-          "attention_beams: more than one share needs a contiguous float32 workspace")
+    if not 1 <= n_beams <= MAX_BEAMS or S % n_beams:
+        raise KernelError(f"attention_beams: {S} sequences in groups of {n_beams} (1 to {MAX_BEAMS})")
+    G, rows = S // n_beams, (S, n_heads * D)
+    if q.shape != rows or out.shape != rows or not q.dtype == cache_slot.dtype == out.dtype:
+        raise KernelError(f"attention_beams: q and out must be {list(rows)}, of the cache's dtype")
+    if not (block_table.dtype == seq_lens.dtype == shared.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= S
+            and block_table.is_contiguous() and seq_lens.is_contiguous() and shared.is_contiguous() and shared.numel() == G):
+        raise KernelError("attention_beams: contiguous int32 block_table [S, max_blocks], seq_lens [S] and shared [S / n_beams] are needed")
+    if n_splits > 1 and (workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous()):
+        raise KernelError("attention_beams: more than one share needs a contiguous float32 workspace")
     _check(_lib().da_attn_beams(_ptr(q), q.stride(0), _ptr(cache_slot), _dt(q), _ptr(block_table), block_table.shape[1], _ptr(seq_lens),
                                 _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), int(window or 0), _ptr(out), out.stride(0),
                                 max(1, int(n_splits)), _ptr(workspace) if n_splits > 1 else None, workspace.numel() if n_splits > 1 else 0,
@@ -1433,10 +1452,13 @@ def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, 
             pairs += sum(min(n - t + i + 1, window or n) for i in range(t)) if t > 1 else min(n, window or n)
         return keys * 2 * Hkv * D * el + 2 * rows * n_heads * D * el, 4 * pairs * n_heads * D
 
-    if ctx.n_beams > 1 and attention_beams_pays(ctx, group, n_heads, Hkv, D, page) and q.stride(0) * el % 16 == 0 and q.data_ptr() % 16 == 0:
+    if (getattr(ctx, "n_beams", 0) > 1 and attention_beams_pays(ctx, group, n_heads, Hkv, D, page) and q.stride(0) * el % 16 == 0
+            and q.data_ptr() % 16 == 0 and cache_slot.data_ptr() % 16 == 0):
         n_splits = beam_splits(nd // ctx.n_beams, ctx.n_beams, n_heads, Hkv, D, bt.shape[1], page)
         ws = ctx.flat("beam_partial", beam_workspace_floats(nd, n_heads, D, n_splits), torch.float32) if n_splits > 1 else None
-        with _timed("attention_beams", *cost(0, nd), "fp32" if el == 4 else "bf16"):
+        nbytes, flops = cost(0, nd)                       # (what a group shares is read once)
+        again = (ctx.n_beams - 1) * sum(ctx.beam_shared_host[group]) * 2 * Hkv * D * el if nbytes and not window else 0
+        with _timed("attention_beams", nbytes - again, flops, "fp32" if el == 4 else "bf16"):
             return attention_beams(q, cache_slot, bt, ctx.seq_lens, ctx.beam_shared[group], ctx.n_beams, n_heads, scale, window, out, n_splits, ws)
     if _MODE == "tuned" and q.dtype == torch.bfloat16 and D % 16 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
         n_splits = decode_splits(nd, n_heads, bt.shape[1], page) if nd else 1

@@ -122,6 +122,7 @@ class StepContext:
         # per cache group int32 [S / n_beams], how many positions those pages hold; the beams' summed log-probabilities, float32 [S]
         self.n_beams = 0
         self.beam_shared: List[torch.Tensor] = []
+        self.beam_shared_host: List[List[int]] = []
         self.beam_scores: torch.Tensor = None
         self.cache = None                              # engine.DeviceCache
         self._arena = None
