@@ -8,25 +8,26 @@
 // 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  The terms of the sum are 32-bit exponentials,
 // summed in 64-bit.
 //
-// Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 2 or 8 segments of 256 logits of a row and leaves each
-// segment's largest logit and, for all of them, the maximum and the sum.  beam_choose_kernel, one workgroup a group, works on
-// what is left.  It finds a key that K entries surely reach, the K-th best of the largest keys of 256 groups of segments (about K + K^2 / 512
-// segments reach it, where their keys come in any order), reads the segments that reach it again, and puts the entries that reach it in order
-// by counting, for each, those in front of it.  Where more reach it than the list holds (equal logits), the key is searched bit by bit, and
-// among equal ones the place.
+// Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 512 or 2,048 logits of a row and leaves their maximum
+// and sum, and the largest of each segment of 64 or 256.  beam_choose_kernel, one workgroup a group, works on what is left, by a bound
+// that K entries surely reach: the best segments of n groups of segments are n entries, and the K-th best of them is such a bound (about K + K^2 / 2n
+// segments reach it).  It reads the segments that reach it again; the entries that do are cut down by bounds of the same
+// kind until they are few, and put in order by counting, for each, those in front of it.  A bound is a key and a place, so that equal logits
+// are cut down too; where more entries reach the first one than the list holds, it is searched bit by bit.
 #include "common.h"
 
 #define BEAM_MAX 64              // beams of a group
 #define BEAM_MAX_KEEP 128        // candidates of a group
-#define SEG 256                  // logits of a segment: 64 lanes, 4 each
-#define SEGS_FEW 2               // segments of a wavefront: few logits, or many
-#define SEGS_MANY 8
+#define LOAD 256                 // logits of a wavefront's load: 64 lanes, 4 each
+#define LOADS_FEW 2              // of a wavefront: few logits, or many
+#define LOADS_MANY 8
 #define STATS_WAVES 4
 #define CHOOSE_THREADS 1024
 #define CHOOSE_WAVES (CHOOSE_THREADS / DA_WAVE)
-#define GROUPS (CHOOSE_THREADS / 4)
-#define HELD 2                   // segments whose keys a thread keeps
-#define LIST 512                 // segments, and entries, that may be looked at one by one
+#define HELD 2                   // segments whose keys a thread, and whose entries a wavefront keeps
+#define SEG_LIST 512             // segments that are read again
+#define LIST 4096                // their entries that reach the bound
+#define LIST_A_THREAD (LIST / CHOOSE_THREADS)
 
 // a 64-bit number that orders like the key; 0 for one that is never chosen
 __device__ __forceinline__ uint64_t ordered64(double v) {
@@ -48,45 +49,61 @@ __device__ __forceinline__ float exp_near(float x) {
   return fmaf(r, rest * 0.693147181f, r);
 }
 
-template <int SEGS>              // of a wavefront
+template <int LOADS, int SEG>    // of a wavefront; logits of a segment
 __global__ void __launch_bounds__(STATS_WAVES * DA_WAVE)
 beam_stats_kernel(const float* __restrict__ logits, long ldl, int V, int n_segs, int n_parts, float* __restrict__ seg_max,
                   float* __restrict__ part_max, double* __restrict__ part_sum) {
   const int lane = threadIdx.x % DA_WAVE, part = blockIdx.x * STATS_WAVES + threadIdx.x / DA_WAVE, row = blockIdx.y;
   if (part >= n_parts) return;
   const float* z = logits + (size_t)row * ldl;
-  const int v0 = part * SEGS * SEG;
-  float x[SEGS][4];
-  if (v0 + SEGS * SEG <= V) {
+  const int v0 = part * LOADS * LOAD;
+  float x[LOADS][4];
+  if (v0 + LOADS * LOAD <= V) {
 #pragma unroll
-    for (int s = 0; s < SEGS; ++s) {
-      const float4_any f = *(const float4_any*)(z + v0 + s * SEG + 4 * lane);
+    for (int s = 0; s < LOADS; ++s) {
+      const float4_any f = *(const float4_any*)(z + v0 + s * LOAD + 4 * lane);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[s][e] = f[e];
     }
   } else {
 #pragma unroll
-    for (int s = 0; s < SEGS; ++s)
+    for (int s = 0; s < LOADS; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int v = v0 + s * SEG + 4 * lane + e;
+        const int v = v0 + s * LOAD + 4 * lane + e;
         x[s][e] = v < V ? z[v] : -INFINITY;
       }
   }
-  float top = -INFINITY, m[SEGS];
+  float top = -INFINITY, m[LOADS];
 #pragma unroll
-  for (int s = 0; s < SEGS; ++s) {                        // (the maximum with a number drops what is none)
-    m[s] = wave_max(fmaxf(fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])), -INFINITY));
+  for (int s = 0; s < LOADS; ++s) {                       // (the maximum with a number drops what is none)
+    m[s] = fmaxf(fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])), -INFINITY);
+    if (SEG == 64) {                                      // 16 lanes
+      m[s] = fmaxf(m[s], dpp_move<0xB1, 0xF>(m[s], m[s]));
+      m[s] = fmaxf(m[s], dpp_move<0x4E, 0xF>(m[s], m[s]));
+      m[s] = fmaxf(m[s], dpp_move<0x141, 0xF>(m[s], m[s]));
+      m[s] = fmaxf(m[s], dpp_move<0x140, 0xF>(m[s], m[s]));
+    } else {
+      m[s] = wave_max(m[s]);
+    }
     top = fmaxf(top, m[s]);
   }
-  float best = m[0];
+  float* row_segs = seg_max + (size_t)row * n_segs;
+  if (SEG == 64) {
+    top = wave_max(top);
 #pragma unroll
-  for (int s = 1; s < SEGS; ++s) best = lane == s ? m[s] : best;
-  if (lane < SEGS && v0 + lane * SEG < V) seg_max[(size_t)row * n_segs + part * SEGS + lane] = best;
+    for (int s = 0; s < LOADS; ++s)
+      if (lane % 16 == 0 && v0 + s * LOAD + 4 * lane < V) row_segs[(part * LOADS + s) * 4 + lane / 16] = m[s];
+  } else {
+    float best = m[0];
+#pragma unroll
+    for (int s = 1; s < LOADS; ++s) best = lane == s ? m[s] : best;
+    if (lane < LOADS && v0 + lane * LOAD < V) row_segs[part * LOADS + lane] = best;
+  }
   double sum = 0.0;
   const bool infinite = top == INFINITY;
 #pragma unroll
-  for (int s = 0; s < SEGS; ++s) {
+  for (int s = 0; s < LOADS; ++s) {
     float e4[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -104,59 +121,95 @@ beam_stats_kernel(const float* __restrict__ logits, long ldl, int V, int n_segs,
 }
 
 struct Chosen {
-  uint64_t key;
-  int place;
+  uint64_t key;                  // 0: none
+  int place;                     // of a segment: its number; of an entry: beam * V + token
 };
 
-__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ bool in_front(uint64_t key, int place, uint64_t other, int other_place) { return key > other || (key == other && place < other_place); }
+__device__ __forceinline__ bool reaches(uint64_t key, int place, const Chosen& bound) { return key > bound.key || (key == bound.key && place <= bound.place); }
+
 template <int CTRL>
-__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
-  const uint32_t lo = (uint32_t)dpp_move_i<CTRL, 0xF>((int)v, (int)v), hi = (uint32_t)dpp_move_i<CTRL, 0xF>((int)(v >> 32), (int)(v >> 32));
-  return (uint64_t)hi << 32 | lo;
+__device__ __forceinline__ void best_of_lanes(Chosen& c) {
+  const uint32_t lo = (uint32_t)dpp_move_i<CTRL, 0xF>((int)c.key, (int)c.key), hi = (uint32_t)dpp_move_i<CTRL, 0xF>((int)(c.key >> 32), (int)(c.key >> 32));
+  const uint64_t k = (uint64_t)hi << 32 | lo;
+  const int p = dpp_move_i<CTRL, 0xF>(c.place, c.place);
+  if (in_front(k, p, c.key, c.place)) { c.key = k; c.place = p; }
+}
+// over groups of 4, 8 or 16 lanes
+__device__ __forceinline__ int sum_of_lanes(int v, int lanes) {
+  v += dpp_move_i<0xB1, 0xF>(v, v);
+  v += dpp_move_i<0x4E, 0xF>(v, v);
+  if (lanes >= 8) v += dpp_move_i<0x141, 0xF>(v, v);
+  if (lanes >= 16) v += dpp_move_i<0x140, 0xF>(v, v);
+  return v;
 }
 
-__device__ __forceinline__ bool stands(uint64_t key, int place, uint64_t least, int last) { return key > least || (key == least && place <= last); }
+// Every thread's best entry: the K-th best of the best entries of groups of `lanes` threads goes to bounds[0] (which keeps what it
+// holds where fewer groups have any), the best to bounds[1].
+__device__ __forceinline__ void bound_of(Chosen best, int lanes, int K, Chosen* group_best, Chosen* bounds) {
+  const int t = threadIdx.x, n_groups = CHOOSE_THREADS / lanes;
+  best_of_lanes<0xB1>(best);
+  best_of_lanes<0x4E>(best);
+  if (lanes >= 8) best_of_lanes<0x141>(best);
+  if (lanes >= 16) best_of_lanes<0x140>(best);
+  if (t % lanes == 0) group_best[t / lanes] = best;
+  __syncthreads();
+  int before = 0;                                       // the threads of a group count, each its part, the groups in front of it
+#pragma unroll 4
+  for (int j = t % lanes; j < n_groups; j += lanes) {
+    const Chosen other = group_best[j];
+    before += in_front(other.key, other.place, best.key, best.place) || (other.key == best.key && other.place == best.place && j < t / lanes);
+  }
+  before = sum_of_lanes(before, lanes);
+  if (before == K - 1 && best.key) bounds[0] = best;    // (the threads of a group write the same)
+  if (before == 0) bounds[1] = best;
+  __syncthreads();
+}
 
-// (least, last) moved up until at most LIST entries stand, and still `keep`: first by the key, then, where more are equal, by
-// the place.  count(least, last): how many stand, the same in all threads.
+// A bound that `keep` entries reach moved up until at most `most` do: first its key, between it and the largest one, then, where
+// more are equal, its place.  count(bound): how many reach it, the same in all threads.
 template <class Count>
-__device__ void narrow(uint64_t& least, int& last, int keep, Count count) {
-  uint64_t hi = 0xffffffffffffffffull;                 // fewer than `keep` reach it
-  int c = LIST + 1;
-  while (c > LIST && hi - least > 1) {
-    const uint64_t mid = least + (hi - least) / 2;
-    const int m = count(mid, last);
-    if (m >= keep) { least = mid; c = m; }
+__device__ void narrow(Chosen& bound, uint64_t largest, int keep, int most, Count count) {
+  uint64_t hi = largest + 1;                            // fewer than `keep` reach it
+  int c = most + 1;
+  while (c > most && hi - bound.key > 1) {
+    const uint64_t mid = bound.key + (hi - bound.key) / 2;
+    const int m = count(Chosen{mid, 0x7fffffff});
+    if (m >= keep) { bound = Chosen{mid, 0x7fffffff}; c = m; }
     else hi = mid;
   }
-  if (c <= LIST) return;
-  for (int a = 0; a < last;) {
-    const int mid = a + (last - a) / 2;
-    if (count(least, mid) >= keep) last = mid;
+  if (c <= most) return;
+  for (int a = 0; a < bound.place;) {
+    const int mid = a + (bound.place - a) / 2;
+    if (count(Chosen{bound.key, mid}) >= keep) bound.place = mid;
     else a = mid + 1;
   }
 }
 
 // magic: 2^32 / n_segs rounded up (0: divide), for fewer than 65,536 segments
+template <int SEG>
 __global__ void __launch_bounds__(CHOOSE_THREADS)
 beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int K, const float* __restrict__ scores, int n_segs,
                    int n_parts, const float* __restrict__ seg_max, const float* __restrict__ part_max, const double* __restrict__ part_sum,
                    float* __restrict__ out_score, int* __restrict__ out_parent, int* __restrict__ out_token, uint32_t magic) {
+  constexpr int SEG_LANES = SEG / 4, SIDE = DA_WAVE / SEG_LANES;      // a segment's lanes, 4 entries each; segments of a wavefront side by side
   __shared__ double base[BEAM_MAX], logsum[BEAM_MAX];     // the score (-inf: no beam); the logarithm of the sum
   __shared__ float top[BEAM_MAX];
-  __shared__ __attribute__((aligned(16))) uint64_t group_best[GROUPS];
-  __shared__ Chosen list[LIST];
-  __shared__ int segs[LIST], counts[CHOOSE_WAVES], n_list[2];
-  __shared__ uint64_t least_of[1];
+  __shared__ Chosen group_best[CHOOSE_THREADS / 4], list[LIST], bounds[2];
+  __shared__ int segs[SEG_LIST], counts[CHOOSE_WAVES], n_list[2];
   const int g = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / DA_WAVE), lane = t % DA_WAVE;
   const size_t row0 = (size_t)g * B;
   const int n = B * n_segs;
+  const int lanes = K <= 32 ? 16 : (K <= 64 ? 8 : 4);     // of a group: 64, 128 or 256 groups, twice as many as candidates
+  // The t-th of what is shared out over the threads: neighbours go to different groups, so that a beam that is ahead of the
+  // others has its segments in all of them.
+  const int t_of = t % lanes * (CHOOSE_THREADS / lanes) + t / lanes;
 
   // ---- asked for together: a thread's first segments, and the partial results of the wavefront's first row
   const float* sm = seg_max + row0 * n_segs;
   float zr[HELD];
 #pragma unroll
-  for (int e = 0; e < HELD; ++e) zr[e] = sm[min(t + e * CHOOSE_THREADS, n - 1)];
+  for (int e = 0; e < HELD; ++e) zr[e] = sm[min(t_of + e * CHOOSE_THREADS, n - 1)];
   for (int b = wave; b < B; b += CHOOSE_WAVES) {
     const float* pm = part_max + (row0 + b) * n_parts;
     const double* ps = part_sum + (row0 + b) * n_parts;
@@ -178,7 +231,7 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     }
   }
   if (t < 2) n_list[t] = 0;
-  if (t == 0) *least_of = 1;
+  if (t < 2) bounds[t] = Chosen{1, 0x7fffffff};           // (every entry that can be chosen reaches it)
   __syncthreads();
   auto key_of = [&](int b, float z) {
     const double x = z == top[b] ? 0.0 : (double)z - (double)top[b];
@@ -195,82 +248,96 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
   };
   auto row_of = [&](int i) { return magic ? (int)__umulhi((uint32_t)i, magic) : i / n_segs; };
 
-  // ---- a key that K entries reach: the K-th best of the largest keys of GROUPS groups of segments
-  uint64_t held[HELD], best = 0;
+  // ---- a bound for the segments' largest entries
+  uint64_t held[HELD];
+  Chosen best{0, 0x7fffffff};
+  auto better = [&](uint64_t k, int i) {
+    if (in_front(k, i, best.key, best.place)) best = Chosen{k, i};
+  };
 #pragma unroll
   for (int e = 0; e < HELD; ++e) {
-    const int i = t + e * CHOOSE_THREADS;
+    const int i = t_of + e * CHOOSE_THREADS;
     held[e] = i < n ? key_of(row_of(i), zr[e]) : 0;
-    best = larger(best, held[e]);
+    better(held[e], i);
   }
-  for (int i = t + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) best = larger(best, key_of(row_of(i), sm[i]));
+  for (int i = t_of + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) better(key_of(row_of(i), sm[i]), i);
+  bound_of(best, lanes, K, group_best, bounds);
+  Chosen bound = bounds[0];
+  const uint64_t largest = bounds[1].key;
+
+  // ---- the segments that reach it
   auto each_seg = [&](auto f) {
 #pragma unroll
-    for (int e = 0; e < HELD; ++e) f(held[e], t + e * CHOOSE_THREADS);      // (one past the end has the key 0)
-    for (int i = t + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) f(key_of(row_of(i), sm[i]), i);
-  };
-  best = larger(best, dpp_u64<0xB1>(best));               // 4 lanes
-  best = larger(best, dpp_u64<0x4E>(best));
-  if (lane % 4 == 0) group_best[t / 4] = best;
-  __syncthreads();
-  {
-    // the four threads of a group count, a quarter each, the groups in front of it
-    int before = 0;
-#pragma unroll 8
-    for (int k = 0; k < GROUPS / 4; ++k) {
-      const int j = 4 * k + t % 4;
-      const uint64_t other = group_best[j];
-      before += other > best || (other == best && j < t / 4);
-    }
-    before += dpp_move_i<0xB1, 0xF>(before, before);
-    before += dpp_move_i<0x4E, 0xF>(before, before);
-    if (before == K - 1 && best > 1) *least_of = best;    // (the four write the same)
-  }
-  __syncthreads();
-  uint64_t least = *least_of;
-
-  // ---- the segments with an entry that reaches it
-  int last = n;
-  auto count_segs = [&](uint64_t lo, int at) {
-    int c = 0;
-    each_seg([&](uint64_t k, int i) { c += stands(k, i, lo, at); });
-    return total(c);
+    for (int e = 0; e < HELD; ++e) f(held[e], t_of + e * CHOOSE_THREADS);      // (one past the end has the key 0)
+    for (int i = t_of + HELD * CHOOSE_THREADS; i < n; i += CHOOSE_THREADS) f(key_of(row_of(i), sm[i]), i);
   };
   auto list_segs = [&]() {
     each_seg([&](uint64_t k, int i) {
-      if (stands(k, i, least, last)) {
+      if (reaches(k, i, bound)) {
         const int at = atomicAdd(&n_list[0], 1);
-        if (at < LIST) segs[at] = i;
+        if (at < SEG_LIST) segs[at] = i;
       }
     });
     __syncthreads();
     return n_list[0];
   };
   int n_found = list_segs();
-  if (n_found > LIST) {
-    narrow(least, last, K, count_segs);
+  if (n_found > SEG_LIST) {
+    narrow(bound, largest, K, SEG_LIST, [&](const Chosen& at) {
+      int c = 0;
+      each_seg([&](uint64_t k, int i) { c += reaches(k, i, at); });
+      return total(c);
+    });
     __syncthreads();
     if (t == 0) n_list[0] = 0;
     __syncthreads();
     n_found = list_segs();
   }
+  // As many entries as segments reach the bound that ends with its segment.
+  if (bound.place < n) bound.place = min(row_of(bound.place) * V + (bound.place - row_of(bound.place) * n_segs + 1) * SEG - 1, (row_of(bound.place) + 1) * V - 1);
 
-  // ---- their entries that reach it: a wavefront a segment
-  int last_place = 0x7fffffff;
+  // ---- their entries that reach it
+  auto keys_of = [&](int j, uint64_t k[4]) {              // of 4 entries of the list's segment SIDE j + lane / SEG_LANES; the first one's place
+    const int at = SIDE * j + lane / SEG_LANES, i = segs[min(at, n_found - 1)], b = row_of(i), v = (i - b * n_segs) * SEG + 4 * (lane % SEG_LANES);
+    const float* z = logits + (row0 + b) * ldl + v;
+    float x[4];
+    if (at < n_found && v + 4 <= V) {
+      const float4_any f = *(const float4_any*)z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = clean(f[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = at < n_found && v + e < V ? clean(z[e]) : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k[e] = key_of(b, x[e]);
+    return b * V + v;
+  };
+  const int n_sides = (n_found + SIDE - 1) / SIDE;
+  uint64_t kept[HELD][4];
+  int place_kept[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    place_kept[h] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) kept[h][e] = 0;
+    if (wave + h * CHOOSE_WAVES < n_sides) place_kept[h] = keys_of(wave + h * CHOOSE_WAVES, kept[h]);
+  }
   auto each_entry = [&](auto f) {
-    for (int j = wave; j < n_found; j += CHOOSE_WAVES) {
-      const int i = __builtin_amdgcn_readfirstlane(segs[j]), b = i / n_segs, v = (i - b * n_segs) * SEG + 4 * lane;
-      const float* z = logits + (row0 + b) * ldl + v;
-      float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = v + e < V ? clean(z[e]) : -INFINITY;
+    for (int h = 0; h < HELD; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(key_of(b, x[e]), b * V + v + e);
+      for (int e = 0; e < 4; ++e) f(kept[h][e], place_kept[h] + e);
+    for (int j = wave + HELD * CHOOSE_WAVES; j < n_sides; j += CHOOSE_WAVES) {
+      uint64_t k[4];
+      const int place = keys_of(j, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(k[e], place + e);
     }
   };
   auto list_entries = [&]() {
     each_entry([&](uint64_t k, int place) {
-      if (stands(k, place, least, last_place)) {
+      if (reaches(k, place, bound)) {
         const int at = atomicAdd(&n_list[1], 1);
         if (at < LIST) list[at] = Chosen{k, place};
       }
@@ -280,9 +347,9 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
   };
   int n_entries = list_entries();
   if (n_entries > LIST) {
-    narrow(least, last_place, K, [&](uint64_t lo, int at) {
+    narrow(bound, largest, K, LIST, [&](const Chosen& at) {
       int c = 0;
-      each_entry([&](uint64_t k, int place) { c += stands(k, place, lo, at); });
+      each_entry([&](uint64_t k, int place) { c += reaches(k, place, at); });
       return total(c);
     });
     __syncthreads();
@@ -291,13 +358,37 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     n_entries = list_entries();
   }
 
-  // ---- in order
-  if (t < n_entries) {
-    const Chosen mine = list[t];
+  // ---- few of them: by bounds of the same kind
+  while (n_entries > CHOOSE_THREADS / lanes * 3 / 2) {
+    Chosen mine[LIST_A_THREAD], first{0, 0x7fffffff};
+#pragma unroll
+    for (int e = 0; e < LIST_A_THREAD; ++e) {
+      const int i = t_of + e * CHOOSE_THREADS;
+      mine[e] = i < n_entries ? list[i] : Chosen{0, 0x7fffffff};
+      if (in_front(mine[e].key, mine[e].place, first.key, first.place)) first = mine[e];
+    }
+    bound_of(first, lanes, K, group_best, bounds);
+    const Chosen next = bounds[0];
+    if (t == 0) n_list[1] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < LIST_A_THREAD; ++e)
+      if (mine[e].key && reaches(mine[e].key, mine[e].place, next)) list[atomicAdd(&n_list[1], 1)] = mine[e];
+    __syncthreads();
+    const int left = n_list[1];
+    if (left == n_entries) break;
+    n_entries = left;
+  }
+
+  // ---- in order: 4 threads an entry count those in front of it
+  for (int i0 = 0; i0 < n_entries; i0 += CHOOSE_THREADS / 4) {
+    const int i = i0 + t / 4;
+    const Chosen mine = list[min(i, n_entries - 1)];
     int r = 0;
 #pragma unroll 4
-    for (int j = 0; j < n_entries; ++j) r += list[j].key > mine.key || (list[j].key == mine.key && list[j].place < mine.place);
-    if (r < K) {
+    for (int j = t % 4; j < n_entries; j += 4) r += in_front(list[j].key, list[j].place, mine.key, mine.place);
+    r = sum_of_lanes(r, 4);
+    if (t % 4 == 0 && i < n_entries && r < K) {
       out_score[(size_t)g * K + r] = (float)unordered64(mine.key);
       out_parent[(size_t)g * K + r] = mine.place / V;
       out_token[(size_t)g * K + r] = mine.place % V;
@@ -310,18 +401,26 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
   }
 }
 
-static long beam_segs(int V) { return ((long)V + SEG - 1) / SEG; }
-// Few logits: as many wavefronts as there can be; many: fewer partial results.
-static int beam_segs_a_wave(long rows, int V) { return rows * beam_segs(V) < 8192 ? SEGS_FEW : SEGS_MANY; }
-static long beam_parts(long rows, int V) {
-  const int s = beam_segs_a_wave(rows, V);
-  return (beam_segs(V) + s - 1) / s;
+// How a call is cut up.  Short segments while a group's fit the threads that keep their keys: of long ones a small vocabulary has fewer
+// than candidates.  Few logits: as many wavefronts as there can be; many: fewer partial results.
+struct Cut {
+  int seg, loads;
+  long n_segs, n_parts;          // of a row
+};
+static Cut beam_cut(long rows, int B, int V) {
+  Cut c;
+  c.seg = (long)B * (((long)V + 63) / 64) <= HELD * CHOOSE_THREADS ? 64 : 256;
+  c.loads = rows * (((long)V + LOAD - 1) / LOAD) < 8192 ? LOADS_FEW : LOADS_MANY;
+  c.n_segs = ((long)V + c.seg - 1) / c.seg;
+  c.n_parts = ((long)V + c.loads * LOAD - 1) / (c.loads * LOAD);
+  return c;
 }
 
 // Scratch of a call, in 32-bit words: the parts' sums (64-bit) and maxima, and the segments' maxima.
-extern "C" int da_beam_select_words(int rows, int V) {
-  if (rows < 0 || V <= 0) return -1;
-  const long words = (long)rows * (3 * beam_parts(rows, V) + beam_segs(V));
+extern "C" int da_beam_select_words(int G, int B, int V) {
+  if (G < 0 || B <= 0 || V <= 0) return -1;
+  const Cut c = beam_cut((long)G * B, B, V);
+  const long words = (long)G * B * (3 * c.n_parts + c.n_segs);
   return words > 0x7fffffffL ? -1 : (int)words;
 }
 
@@ -332,7 +431,8 @@ extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V
   DA_REQUIRE(K > 0 && K <= BEAM_MAX_KEEP, "beam_select: %d candidates (1 to %d)", K, BEAM_MAX_KEEP);
   if (G == 0) return 0;
   const long rows = (long)G * B;
-  const int n_parts = (int)beam_parts(rows, V), n_segs = (int)beam_segs(V);
+  const Cut cut = beam_cut(rows, B, V);
+  const int n_parts = (int)cut.n_parts, n_segs = (int)cut.n_segs;
   const long words = rows * (3L * n_parts + n_segs);
   DA_REQUIRE(rows <= 65535, "beam_select: %ld rows (at most 65,535)", rows);
   DA_REQUIRE(scratch && (uintptr_t)scratch % 8 == 0 && scratch_words >= words, "beam_select: %ld words of scratch on 8 bytes are needed, found %ld", words, scratch_words);
@@ -340,15 +440,22 @@ extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V
   float* part_max = scratch + 2 * rows * n_parts;
   float* seg_max = part_max + rows * n_parts;
   const dim3 grid(da_ceil_div(n_parts, STATS_WAVES), (unsigned)rows), block(STATS_WAVES * DA_WAVE);
-  if (beam_segs_a_wave(rows, V) == SEGS_FEW)
-    hipLaunchKernelGGL((beam_stats_kernel<SEGS_FEW>), grid, block, 0, (hipStream_t)stream, logits, ldl, V, n_segs, n_parts, seg_max, part_max, part_sum);
-  else
-    hipLaunchKernelGGL((beam_stats_kernel<SEGS_MANY>), grid, block, 0, (hipStream_t)stream, logits, ldl, V, n_segs, n_parts, seg_max, part_max, part_sum);
+#define DA_STATS(LOADS, SEG) \
+  hipLaunchKernelGGL((beam_stats_kernel<LOADS, SEG>), grid, block, 0, (hipStream_t)stream, logits, ldl, V, n_segs, n_parts, seg_max, part_max, part_sum)
+  if (cut.seg == 64 && cut.loads == LOADS_FEW) DA_STATS(LOADS_FEW, 64);
+  else if (cut.seg == 64) DA_STATS(LOADS_MANY, 64);
+  else if (cut.loads == LOADS_FEW) DA_STATS(LOADS_FEW, 256);
+  else DA_STATS(LOADS_MANY, 256);
+#undef DA_STATS
   DA_CHECK_LAUNCH("beam_select (sums)");
   // i * magic / 2^32 is i / n_segs while i < 2^16 and n_segs < 2^16: the product's error, i * (magic * n_segs - 2^32) / n_segs / 2^32, is below i / 2^32
   const uint32_t magic = (long)B * n_segs < 65536 && n_segs > 1 ? (uint32_t)(((1ull << 32) + n_segs - 1) / n_segs) : 0;
-  hipLaunchKernelGGL(beam_choose_kernel, dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts,
-                     seg_max, part_max, part_sum, out_score, out_parent, out_token, magic);
+#define DA_CHOOSE(SEG) \
+  hipLaunchKernelGGL((beam_choose_kernel<SEG>), dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts, \
+                     seg_max, part_max, part_sum, out_score, out_parent, out_token, magic)
+  if (cut.seg == 64) DA_CHOOSE(64);
+  else DA_CHOOSE(256);
+#undef DA_CHOOSE
   DA_CHECK_LAUNCH("beam_select (choice)");
   return 0;
 }

@@ -247,7 +247,7 @@ class BeamSearch:
         n, dev = len(group), logits.device
         out = (torch.empty(n, self.n_keep, device=dev), torch.empty(n, self.n_keep, dtype=torch.int32, device=dev),
                torch.empty(n, self.n_keep, dtype=torch.int32, device=dev))
-        ws = torch.empty(ops.beam_select_floats(*logits.shape), device=dev)
+        ws = torch.empty(ops.beam_select_floats(n, 1, logits.shape[1]), device=dev)
         chosen = ops.beam_select(logits, torch.zeros(n, device=dev), 1, *out, ws)
         for w, c in zip(group, self._candidates(chosen)):
             w.group.take(c)

@@ -334,7 +334,7 @@ class StepRunner:
         per = ctx.n_seqs // beams.n_beams
         out = (ctx.buf("beam_out_scores", per, beams.n_keep, torch.float32), ctx.buf("beam_out_parents", per, beams.n_keep, torch.int32),
                ctx.buf("beam_out_tokens", per, beams.n_keep, torch.int32))
-        ws = ctx.flat("beam_select", ops.beam_select_floats(*logits.shape), torch.float32)
+        ws = ctx.flat("beam_select", ops.beam_select_floats(logits.shape[0], beams.n_beams, logits.shape[1]), torch.float32)
         return ops.beam_select(logits, ctx.beam_scores, beams.n_beams, *out, ws)
 
     def _run_eager(self, entries, order, starts, sample_records, beams=None):

@@ -184,7 +184,7 @@ _ARGTYPES = {
     "da_rglru_decode": [_VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, ctypes.c_long, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP],
     "da_rglru_portion": [_VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, ctypes.c_long, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I,
                          _VP, ctypes.c_long, _VP],
-    "da_beam_select_words": [_I, _I],
+    "da_beam_select_words": [_I, _I, _I],
     "da_beam_select": [_VP, ctypes.c_long, _I, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, ctypes.c_long, _VP],
     "da_state_reorder": [_VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP],
     "da_attn_beams_takes": [_I, _I],
@@ -849,10 +849,10 @@ def sample(logits: torch.Tensor, params: torch.Tensor, out_tokens: torch.Tensor)
 MAX_BEAMS, MAX_CANDIDATES = 64, 128     # of a group (csrc/beam_select.hip)
 
 
-def beam_select_floats(n_rows: int, vocab: int) -> int:
-    """32-bit words of scratch that ``beam_select`` needs for logits [n_rows, vocab]."""
-    n = int(_lib().da_beam_select_words(int(n_rows), int(vocab)))
-    _need(n >= 0, f"beam_select: {n_rows} rows of {vocab} logits are too many")
+def beam_select_floats(n_rows: int, n_beams: int, vocab: int) -> int:
+    """32-bit words of scratch that ``beam_select`` needs for logits [n_rows, vocab] in groups of ``n_beams``."""
+    n = int(_lib().da_beam_select_words(int(n_rows) // max(1, int(n_beams)), int(n_beams), int(vocab)))
+    _need(n >= 0, f"beam_select: {n_rows} rows of {vocab} logits in groups of {n_beams}")
     return n
 
 

@@ -39,7 +39,7 @@ def plain_select(logits, scores, B, K):
 
 def select(logits, scores, B, K):
     G = logits.shape[0] // B
-    ws = torch.full((ops.beam_select_floats(logits.shape[0], logits.shape[1]),), math.nan, device=DEV)
+    ws = torch.full((ops.beam_select_floats(logits.shape[0], B, logits.shape[1]),), math.nan, device=DEV)
     out = (torch.full((G, K), math.nan, device=DEV), torch.full((G, K), -7, dtype=torch.int32, device=DEV),
            torch.full((G, K), -7, dtype=torch.int32, device=DEV))
     got = ops.beam_select(logits, scores, B, *out, ws)
@@ -129,7 +129,7 @@ def test_a_large_score_does_not_make_neighbouring_logits_equal():
 def test_refusals_of_the_choice():
     logits, scores = torch.zeros(6, 40, device=DEV), torch.zeros(6, device=DEV)
     out = (torch.zeros(2, 4, device=DEV), torch.zeros(2, 4, dtype=torch.int32, device=DEV), torch.zeros(2, 4, dtype=torch.int32, device=DEV))
-    ws = torch.zeros(ops.beam_select_floats(6, 40), device=DEV)
+    ws = torch.zeros(ops.beam_select_floats(6, 3, 40), device=DEV)
     ops.beam_select(logits, scores, 3, *out, ws)
     for bad in (dict(logits=logits.bfloat16()), dict(logits=logits.t()), dict(scores=scores[:5]), dict(n_beams=4), dict(n_beams=0), dict(n_beams=65),
                 dict(out_scores=out[0].double()), dict(out_parents=out[1].long()), dict(out_tokens=out[2][:1]), dict(out_scores=out[0].t()),
