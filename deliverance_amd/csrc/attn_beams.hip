@@ -23,8 +23,9 @@
 #define BEAMS_MAX_D 256
 #define CHUNK 64
 #define ROWS 16                  // of a workgroup
-#define BEAM_WAVES 4
 
+template <int N>
+struct Int { static const int value = N; };
 struct Yes { static const bool value = true; };
 struct No { static const bool value = false; };
 
@@ -60,8 +61,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // DK: head size in steps of 32, rounded up to a power of two.  STEP: keys whose loads are under way together.
-template <typename T, int DK, int STEP>
-__global__ void __launch_bounds__(BEAM_WAVES * DA_WAVE)
+template <typename T, int DK, int STEP, int WAVES>
+__global__ void __launch_bounds__(WAVES * DA_WAVE)
 attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache, const int* __restrict__ block_table, int max_blocks,
                   const int* __restrict__ seq_lens, const int* __restrict__ shared, int B, int Hq, int Hkv, int D, int page, float scale,
                   int window, T* __restrict__ out, int out_ld, int splits, float* __restrict__ partial) {
@@ -71,8 +72,8 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   constexpr int KP = STEP / 16;                         // pieces of 16 keys
   constexpr int VP = F32 ? STEP / 16 : STEP / 32;       // value loads a dimension: 4 keys (32-bit) or 8 a lane
   constexpr int SPAN = F32 ? 4 : 8;                     // consecutive keys of a lane
-  __shared__ float acc_lds[BEAM_WAVES][DMAX][ROWS + 1];
-  __shared__ float m_lds[BEAM_WAVES][ROWS], l_lds[BEAM_WAVES][ROWS];
+  __shared__ float acc_lds[WAVES][DMAX][ROWS + 1];
+  __shared__ float m_lds[WAVES][ROWS], l_lds[WAVES][ROWS];
 
   const int t = threadIdx.x, lane = t % DA_WAVE, wave = __builtin_amdgcn_readfirstlane(t / DA_WAVE);
   const int col = lane % 16, quad = lane / 16;
@@ -117,35 +118,67 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   const T* const kbase = cache + (size_t)hk * page * D;
   const T* const vbase = cache + (size_t)(Hkv + hk) * page * D;
 
-  for (int item = item0 + wave; item < item1; item += BEAM_WAVES) {
-    // which chunk of whose table (own < 0: of all)
-    int chunk = shared0 + item, mine = -1, src = first_live, first = 0, last = 0x7fffffff;
+  // Which chunk of whose table an item is (mine < 0: of all), and which of its positions are seen.
+  struct Item {
+    int mine, c0, first, last;
+  };
+  auto item_at = [&](int item) {
+    Item it{-1, (shared0 + item) * CHUNK, 0, 0};
+    it.first = it.c0;
+    it.last = it.c0 + CHUNK - 1;
     if (item >= n_shared) {
       const int left = item - n_shared;
-      mine = __builtin_popcountll(__builtin_amdgcn_ballot_w64(own_to <= left));
-      mine = min(mine, b1);
-      chunk = __builtin_amdgcn_readlane(own0, mine) + left - (__builtin_amdgcn_readlane(own_to, mine) - __builtin_amdgcn_readlane(own, mine));
+      it.mine = min((int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own_to <= left)), b1);
+      int chunk = __builtin_amdgcn_readlane(own0, it.mine) + left - (__builtin_amdgcn_readlane(own_to, it.mine) - __builtin_amdgcn_readlane(own, it.mine));
       if (chunk >= shared0) chunk += n_shared;
-      src = mine;
-      first = max(chunk * CHUNK, __builtin_amdgcn_readlane(lo_b, mine));
-      last = min(chunk * CHUNK + CHUNK, __builtin_amdgcn_readlane(n_b, mine)) - 1;
-    } else {
-      first = chunk * CHUNK;
-      last = first + CHUNK - 1;
+      it.c0 = chunk * CHUNK;
+      it.first = max(it.c0, __builtin_amdgcn_readlane(lo_b, it.mine));
+      it.last = min(it.c0 + CHUNK, __builtin_amdgcn_readlane(n_b, it.mine)) - 1;
     }
-    const int* bt = block_table + (size_t)(s0 + src) * max_blocks;
+    return it;
+  };
+  // The pages of a lane's keys and values: keys (and groups of SPAN values) that nobody sees are read from a place that somebody does.
+  constexpr int KI = F32 ? 4 : 2;                       // pages a lane has to look up: bfloat16: a group of 8 keys every 32
+  struct Pages {
+    int k[KI], v[KI];
+  };
+  auto pages_of = [&](const Item& it) {
+    const int* bt = block_table + (size_t)(s0 + (it.mine < 0 ? first_live : it.mine)) * max_blocks;
+    Pages p;
+#pragma unroll
+    for (int j = 0; j < KI; ++j) {
+      const int kj = it.c0 + CHUNK / KI * j + (F32 ? col : 8 * (col / 4)), vj = it.c0 + CHUNK / KI * j + SPAN * quad;
+      p.k[j] = bt[max(it.first, min(it.last, kj)) >> lg];
+      p.v[j] = bt[max(it.first, min(it.last, vj)) >> lg];
+    }
+    return p;
+  };
+
+  Item now = item_at(min(item0 + wave, max(items - 1, 0)));
+  Pages pages;
+  if (item0 + wave < item1) pages = pages_of(now);
+  for (int item = item0 + wave; item < item1; item += WAVES) {
+    const int mine = now.mine, c0 = now.c0, first = now.first, last = now.last;
+    const Pages here = pages;
+    if (item + WAVES < item1) {                    // the next item's pages travel beside this one's keys and values
+      now = item_at(item + WAVES);
+      pages = pages_of(now);
+    }
     const bool takes = mine < 0 || mine == beam;
 
-    auto step = [&](int h0, auto cut_tag) {
+    auto step = [&](auto at_tag, auto cut_tag) {
+      constexpr int AT = decltype(at_tag)::value;       // the step's place in the chunk
       constexpr bool CUT = decltype(cut_tag)::value;
-      // ---- every load of the step, then the arithmetic.  A lane's keys of the first product lie in one group of 8 (bfloat16), or are one
-      // key a piece; keys and values that nobody sees are read from a place that somebody does.
+      const int h0 = c0 + AT;
+      if (CUT && (h0 > last || h0 + STEP <= first)) return;
+      // ---- every load of the step, then the arithmetic
       uint4 kf[KP][QS], vf[VP][DV];
 #pragma unroll
       for (int j = 0; j < KP; ++j) {
         const int key = h0 + (F32 ? 16 * j + col : 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4);
-        const int seen = CUT ? max(first, min(last, key)) : key;
-        const T* kp = kbase + (size_t)(uint32_t)max(bt[seen >> lg], 0) * page_elems + (size_t)(seen & pmask) * D;
+        // (a key that nobody sees: the one of its group's page that the page was looked up for)
+        const int seen = CUT && (key < first || key > last) ? max(first, min(last, F32 ? key : key & ~7)) : key;
+        const T* kp = kbase + (size_t)(uint32_t)max(here.k[(AT + 16 * j) / (CHUNK / KI)], 0) * page_elems + (size_t)(seen & pmask) * D;
 #pragma unroll
         for (int k = 0; k < QS; ++k) {
           const int d = F32 ? 16 * k + 4 * quad : 32 * k + 8 * quad;
@@ -160,9 +193,8 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
 #pragma unroll
       for (int j = 0; j < VP; ++j) {
         const int k0 = h0 + 4 * SPAN * j + SPAN * quad;  // the lane's first key
-        const bool any = !CUT || (k0 <= last && k0 + SPAN - 1 >= first);
-        const int at = any ? k0 : (first & ~(SPAN - 1));
-        const T* vp = vbase + (size_t)(uint32_t)max(bt[at >> lg], 0) * page_elems + (size_t)col * page + (at & pmask);
+        const int at = CUT ? max(first, min(last, k0)) & ~(SPAN - 1) : k0;
+        const T* vp = vbase + (size_t)(uint32_t)max(here.v[(AT + 4 * SPAN * j) / (CHUNK / KI)], 0) * page_elems + (size_t)col * page + (at & pmask);
 #pragma unroll
         for (int i = 0; i < DV; ++i) {
           vf[j][i] = *(const uint4*)vp;
@@ -259,52 +291,59 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
         for (int x = 0; x < 4; ++x) acc[i][x] = !CUT || takes ? o[x] : acc[i][x];
       }
     };
-    if (mine < 0) {
-#pragma unroll 1
-      for (int h0 = first; h0 <= last; h0 += STEP) step(h0, No{});
-    } else {
-#pragma unroll 1
-      for (int h0 = chunk * CHUNK + (first % CHUNK) / STEP * STEP; h0 <= last; h0 += STEP) step(h0, Yes{});
-    }
+    auto all_steps = [&](auto cut_tag) {
+      step(Int<0>{}, cut_tag);
+      if constexpr (STEP < 64) step(Int<STEP>{}, cut_tag);
+      if constexpr (STEP < 32) {
+        step(Int<2 * STEP>{}, cut_tag);
+        step(Int<3 * STEP>{}, cut_tag);
+      }
+    };
+    if (mine < 0) all_steps(No{});
+    else all_steps(Yes{});
   }
 
   // ---- the wavefronts' results joined
   l += __shfl_xor(l, 16, DA_WAVE);
   l += __shfl_xor(l, 32, DA_WAVE);
-  if (len <= 0) l = 0.f;                                // (a place without a beam went along in the shared chunks)
   if (quad == 0) {
-    m_lds[wave][col] = len > 0 ? m : -INFINITY;
-    l_lds[wave][col] = l;
+    m_lds[wave][col] = len > 0 ? m : -INFINITY;         // (a place without a beam went along in the shared chunks)
+    l_lds[wave][col] = len > 0 ? l : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < DV; ++i)
 #pragma unroll
     for (int x = 0; x < 4; ++x) acc_lds[wave][16 * i + 4 * quad + x][col] = len > 0 ? acc[i][x] : 0.f;
   __syncthreads();
-  for (int i = t; i < ROWS * D; i += BEAM_WAVES * DA_WAVE) {
-    const int row = i / D, d = i - row * D;
-    if (r0 + row >= R) break;
-    float mm = -INFINITY;
+  // 16 threads a row, 16 dimensions that follow each other
+  const int row = t / 16 % ROWS, of_row = r0 + row;
+  if (of_row >= R) return;
+  float w[WAVES], mm = -INFINITY, ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < BEAM_WAVES; ++w) mm = fmaxf(mm, m_lds[w][row]);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, o = 0.f;
+  for (int v = 0; v < WAVES; ++v) mm = fmaxf(mm, m_lds[v][row]);
+  const float m_use = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-    for (int w = 0; w < BEAM_WAVES; ++w) {
-      const float a = exp_of_2(m_lds[w][row] - m_use);
-      ll += a * l_lds[w][row];
-      o += a * acc_lds[w][d][row];
-    }
-    const int bm = (r0 + row) / ratio, hd = hk * ratio + (r0 + row - bm * ratio);
-    if (splits == 1) from_f32(out + (size_t)(s0 + bm) * out_ld + (size_t)hd * D + d, ll > 0.f || ll != ll ? o / ll : 0.f);
-    else {
-      float* p = partial + (((size_t)(s0 + bm) * Hq + hd) * splits + z) * (D + 2);
-      p[d] = o;
-      if (d == 0) {
-        p[D] = mm;
-        p[D + 1] = ll;
-      }
-    }
+  for (int v = 0; v < WAVES; ++v) {
+    w[v] = exp_of_2(m_lds[v][row] - m_use);
+    ll += w[v] * l_lds[v][row];
+  }
+  const int bm = of_row / ratio, hd = hk * ratio + (of_row - bm * ratio);
+  const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+  T* o_row = out + (size_t)(s0 + bm) * out_ld + (size_t)hd * D;
+  float* p_row = partial + (((size_t)(s0 + bm) * Hq + hd) * splits + z) * (D + 2);
+#pragma unroll
+  for (int k = 0; k < DMAX; k += WAVES * DA_WAVE / ROWS) {
+    const int d = k + t / (16 * ROWS) * 16 + t % 16;
+    if (d >= D) break;
+    float o = 0.f;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) o += w[v] * acc_lds[v][d][row];
+    if (splits == 1) from_f32(o_row + d, o * inv);
+    else p_row[d] = o;
+  }
+  if (splits > 1 && t < 16 * ROWS && t % 16 == 0) {
+    p_row[D] = mm;
+    p_row[D + 1] = ll;
   }
 }
 
@@ -345,19 +384,34 @@ extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int ma
   if (G <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_blocks <= 0 || page <= 0) return 1;
   const long groups = (long)G * Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS);
   const long chunks = ((long)max_blocks * page + CHUNK - 1) / CHUNK;
-  long n = 512 / groups;
-  if (n > chunks / BEAM_WAVES) n = chunks / BEAM_WAVES;
-  return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
+  // one workgroup a compute unit; a second kernel does not pay for short sequences
+  long n = chunks < 8 ? 1 : 256 / groups;
+  if (n > chunks / 2) n = chunks / 2;
+  return n < 1 ? 1 : (n > DA_WAVE ? DA_WAVE : (int)n);
+}
+
+// Wavefronts of a workgroup.  8 where there is one workgroup a compute unit, which they fill by themselves: 8 x 8 beams of 25 heads over 1,003 positions
+// 17.3 us for 20.1, 24 beams of 7 heads over 3,456 11.5 for 13.6.  4 where more share one, and where each has so many chunks that 4 wavefronts
+// keep the memory busy: 4 x 4 beams over 32,701 positions, 64 chunks each, 104 us for 113 (26 chunks each: 29.2 for 27.5).
+static int beam_waves(int G, int B, int Hq, int Hkv, int splits, int max_blocks, int page) {
+  const long groups = (long)G * Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS);
+  return groups * splits > 256 || (long)max_blocks * page / CHUNK >= 48L * splits ? 4 : 8;
 }
 
 template <typename T, int DK, int STEP>
 static void beams_launch(hipStream_t s, const void* q, int q_ld, const void* cache, const int* block_table, int max_blocks, const int* seq_lens,
                          const int* shared, int G, int B, int Hq, int Hkv, int D, int page, float scale, int window, void* out, int out_ld,
                          int splits, float* partial) {
-  const int blocks = da_ceil_div((long)B * (Hq / Hkv), ROWS);
-  hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP>), dim3(Hkv * blocks, G, splits), dim3(BEAM_WAVES * DA_WAVE), 0, s, (const T*)q, q_ld,
-                     (const T*)cache, block_table, max_blocks, seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits,
-                     partial);
+  const dim3 grid(Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS), G, splits);
+  if constexpr (DK < 8) {                               // (head sizes above 128 have registers for 4 wavefronts only)
+    if (beam_waves(G, B, Hq, Hkv, splits, max_blocks, page) == 8) {
+      hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP, 8>), grid, dim3(8 * DA_WAVE), 0, s, (const T*)q, q_ld, (const T*)cache, block_table,
+                         max_blocks, seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits, partial);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP, 4>), grid, dim3(4 * DA_WAVE), 0, s, (const T*)q, q_ld, (const T*)cache, block_table, max_blocks,
+                     seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits, partial);
 }
 
 extern "C" int da_attn_beams(const void* q, int q_ld, const void* cache, int dtype, const int* block_table, int max_blocks, const int* seq_lens,
@@ -379,7 +433,7 @@ extern "C" int da_attn_beams(const void* q, int q_ld, const void* cache, int dty
   if (dtype == DA_F32) {
     if (D <= 32) DA_BEAMS(float, 1, 32);
     else if (D <= 64) DA_BEAMS(float, 2, 32);
-    else if (D <= 128) DA_BEAMS(float, 4, 32);
+    else if (D <= 128) DA_BEAMS(float, 4, 16);
     else DA_BEAMS(float, 8, 16);
   } else {
     if (D <= 32) DA_BEAMS(bf16_t, 1, 64);
