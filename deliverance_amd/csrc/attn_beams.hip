@@ -22,7 +22,7 @@
 #define BEAMS_MAX 64             // beams of a group
 #define BEAMS_MAX_D 256
 #define CHUNK 64
-#define ROWS 16                  // of a workgroup
+#define TILE 16                  // rows of a matrix product
 
 template <int N>
 struct Int { static const int value = N; };
@@ -61,7 +61,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // DK: head size in steps of 32, rounded up to a power of two.  STEP: keys whose loads are under way together.
-template <typename T, int DK, int STEP, int WAVES>
+// RT: tiles of 16 rows.
+template <typename T, int DK, int STEP, int WAVES, int RT>
 __global__ void __launch_bounds__(WAVES * DA_WAVE)
 attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache, const int* __restrict__ block_table, int max_blocks,
                   const int* __restrict__ seq_lens, const int* __restrict__ shared, int B, int Hq, int Hkv, int D, int page, float scale,
@@ -72,6 +73,7 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   constexpr int KP = STEP / 16;                         // pieces of 16 keys
   constexpr int VP = F32 ? STEP / 16 : STEP / 32;       // value loads a dimension: 4 keys (32-bit) or 8 a lane
   constexpr int SPAN = F32 ? 4 : 8;                     // consecutive keys of a lane
+  constexpr int ROWS = TILE * RT;
   __shared__ float acc_lds[WAVES][DMAX][ROWS + 1];
   __shared__ float m_lds[WAVES][ROWS], l_lds[WAVES][ROWS];
 
@@ -85,15 +87,21 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   const uint32_t page_elems = 2u * (uint32_t)(Hkv * page * D);
   const int cap = max_blocks * page;                    // (a longer length would lead out of the table)
 
-  // a beam a lane: its length; then the query rows, the right operand (row r of the group is column r - r0)
+  // a beam a lane: its length; then the query rows, the right operand (row r of the group is column (r - r0) % 16 of tile (r - r0) / 16)
   const int n_raw = seq_lens[s0 + (lane < B ? lane : 0)], shared_g = shared[g];
-  const int r = r0 + col, rr = min(r, R - 1), beam = rr / ratio, head = hk * ratio + (rr - beam * ratio);
-  uint4 qf[QS];
+  int beam[RT];
+  uint4 qf[RT][QS];
 #pragma unroll
-  for (int k = 0; k < QS; ++k) {
-    const int d = F32 ? 16 * k + 4 * quad : 32 * k + 8 * quad;
-    qf[k] = make_uint4(0, 0, 0, 0);
-    if (d < D && r < R) qf[k] = *(const uint4*)(q + (size_t)(s0 + beam) * q_ld + (size_t)head * D + d);
+  for (int y = 0; y < RT; ++y) {
+    const int r = r0 + TILE * y + col, rr = min(r, R - 1);
+    beam[y] = rr / ratio;
+    const int head = hk * ratio + (rr - beam[y] * ratio);
+#pragma unroll
+    for (int k = 0; k < QS; ++k) {
+      const int d = F32 ? 16 * k + 4 * quad : 32 * k + 8 * quad;
+      qf[y][k] = make_uint4(0, 0, 0, 0);
+      if (d < D && r < R) qf[y][k] = *(const uint4*)(q + (size_t)(s0 + beam[y]) * q_ld + (size_t)head * D + d);
+    }
   }
   const int n_b = lane < B ? max(0, min(n_raw, cap)) : 0, lo_b = window > 0 ? max(0, n_b - window) : 0;
   const uint64_t alive = __builtin_amdgcn_ballot_w64(n_b > 0);
@@ -108,13 +116,20 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   const int n_shared = shared1 - shared0, items = n_shared + __builtin_amdgcn_readlane(own_to, DA_WAVE - 1);
   const int per = (items + splits - 1) / splits;
   const int item0 = z * per, item1 = min(items, item0 + per);
-  const int len_of_beam = __shfl(n_b, beam, DA_WAVE), lo = __shfl(lo_b, beam, DA_WAVE), len = r < R ? len_of_beam : 0;
   const float scale2 = scale * 1.4426950408889634f;
-
-  floatx4 acc[DV];
+  int len[RT], lo[RT];
+  floatx4 acc[RT][DV];
+  float m[RT], l[RT];
 #pragma unroll
-  for (int i = 0; i < DV; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int y = 0; y < RT; ++y) {
+    const int n = __shfl(n_b, beam[y], DA_WAVE);
+    lo[y] = __shfl(lo_b, beam[y], DA_WAVE);
+    len[y] = r0 + TILE * y + col < R ? n : 0;
+    m[y] = -INFINITY;
+    l[y] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DV; ++i) acc[y][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
   const T* const kbase = cache + (size_t)hk * page * D;
   const T* const vbase = cache + (size_t)(Hkv + hk) * page * D;
 
@@ -164,8 +179,6 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
       now = item_at(item + WAVES);
       pages = pages_of(now);
     }
-    const bool takes = mine < 0 || mine == beam;
-
     auto step = [&](auto at_tag, auto cut_tag) {
       constexpr int AT = decltype(at_tag)::value;       // the step's place in the chunk
       constexpr bool CUT = decltype(cut_tag)::value;
@@ -202,93 +215,97 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      floatx4 sc[KP];
 #pragma unroll
-      for (int j = 0; j < KP; ++j) sc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int y = 0; y < RT; ++y) {
+        const bool takes = mine < 0 || mine == beam[y];
+        floatx4 sc[KP];
 #pragma unroll
-      for (int k = 0; k < QS; ++k)
+        for (int j = 0; j < KP; ++j) sc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < KP; ++j) {
-          if (F32) {
-            const uint32_t ka[4] = {kf[j][k].x, kf[j][k].y, kf[j][k].z, kf[j][k].w}, qa[4] = {qf[k].x, qf[k].y, qf[k].z, qf[k].w};
+        for (int k = 0; k < QS; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka[i]), __uint_as_float(qa[i]), sc[j], 0, 0, 0);
-          } else {
-            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[j][k]), __builtin_bit_cast(bf16x8_t, qf[k]), sc[j], 0, 0, 0);
-          }
-        }
-      // ---- the lane's keys: four a piece, of column col's row
-      float e[KP][4], top = -INFINITY;
+          for (int j = 0; j < KP; ++j) {
+            if (F32) {
+              const uint32_t ka[4] = {kf[j][k].x, kf[j][k].y, kf[j][k].z, kf[j][k].w}, qa[4] = {qf[y][k].x, qf[y][k].y, qf[y][k].z, qf[y][k].w};
 #pragma unroll
-      for (int j = 0; j < KP; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[j][i] = sc[j][i] * scale2;
-          if (CUT) {
-            const int key = h0 + (F32 ? 16 * j + 4 * quad + i : 32 * (j / 2) + 8 * quad + 4 * (j % 2) + i);
-            e[j][i] = takes && key >= lo && key < len ? e[j][i] : -INFINITY;
-          }
-          top = fmaxf(top, e[j][i]);
-        }
-      const float m_new = fmaxf(m, quad_max(top)), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp_of_2(m - m_use);
-      m = m_new;
-      float add = 0.f;
-#pragma unroll
-      for (int j = 0; j < KP; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[j][i] = exp_of_2(e[j][i] - m_use);
-          add += e[j][i];
-        }
-      l = l * alpha + add;
-      uint4 hi[VP], lw[VP];                             // bfloat16: the weights' two parts
-      if (!F32) {
-#pragma unroll
-        for (int j = 0; j < VP; ++j) {
-          uint32_t h4[4], l4[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float x = e[2 * j + w / 2][2 * (w % 2)], y = e[2 * j + w / 2][2 * (w % 2) + 1];
-            h4[w] = pack2_bf16(x, y);
-            l4[w] = pack2_bf16(x - __uint_as_float(h4[w] << 16), y - __uint_as_float(h4[w] & 0xffff0000u));
-          }
-          hi[j] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-          lw[j] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < DV; ++i) {
-        floatx4 o;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[x] = acc[i][x] * alpha;
-#pragma unroll
-        for (int j = 0; j < VP; ++j) {
-          uint32_t v4[4] = {vf[j][i].x, vf[j][i].y, vf[j][i].z, vf[j][i].w};
-          if (CUT) {                                    // positions that are not seen may hold anything
-            const int k0 = h0 + 4 * SPAN * j + SPAN * quad;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if (F32) v4[w] = (k0 + w >= first && k0 + w <= last) ? v4[w] : 0u;
-              else {
-                const int ka = k0 + 2 * w;
-                v4[w] &= ((ka >= first && ka <= last) ? 0x0000ffffu : 0u) | ((ka + 1 >= first && ka + 1 <= last) ? 0xffff0000u : 0u);
-              }
+              for (int i = 0; i < 4; ++i)
+                sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka[i]), __uint_as_float(qa[i]), sc[j], 0, 0, 0);
+            } else {
+              sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[j][k]), __builtin_bit_cast(bf16x8_t, qf[y][k]), sc[j], 0, 0, 0);
             }
           }
-          if (F32) {
+        // ---- the lane's keys: four a piece, of column col's row
+        float e[KP][4], top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v4[x]), e[j][x], o, 0, 0, 0);
-          } else {
-            const uint4 v = make_uint4(v4[0], v4[1], v4[2], v4[3]);
-            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, hi[j]), o, 0, 0, 0);
-            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, lw[j]), o, 0, 0, 0);
+        for (int j = 0; j < KP; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[j][i] = sc[j][i] * scale2;
+            if (CUT) {
+              const int key = h0 + (F32 ? 16 * j + 4 * quad + i : 32 * (j / 2) + 8 * quad + 4 * (j % 2) + i);
+              e[j][i] = takes && key >= lo[y] && key < len[y] ? e[j][i] : -INFINITY;
+            }
+            top = fmaxf(top, e[j][i]);
+          }
+        const float m_new = fmaxf(m[y], quad_max(top)), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp_of_2(m[y] - m_use);
+        m[y] = m_new;
+        float add = 0.f;
+#pragma unroll
+        for (int j = 0; j < KP; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[j][i] = exp_of_2(e[j][i] - m_use);
+            add += e[j][i];
+          }
+        l[y] = l[y] * alpha + add;
+        uint4 hi[VP], lw[VP];                           // bfloat16: the weights' two parts
+        if (!F32) {
+#pragma unroll
+          for (int j = 0; j < VP; ++j) {
+            uint32_t h4[4], l4[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float x0 = e[2 * j + w / 2][2 * (w % 2)], x1 = e[2 * j + w / 2][2 * (w % 2) + 1];
+              h4[w] = pack2_bf16(x0, x1);
+              l4[w] = pack2_bf16(x0 - __uint_as_float(h4[w] << 16), x1 - __uint_as_float(h4[w] & 0xffff0000u));
+            }
+            hi[j] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+            lw[j] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
           }
         }
-        // (a column that takes no part keeps its sums: zero times another beam's infinite value is no number)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[i][x] = !CUT || takes ? o[x] : acc[i][x];
+        for (int i = 0; i < DV; ++i) {
+          floatx4 o;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[x] = acc[y][i][x] * alpha;
+#pragma unroll
+          for (int j = 0; j < VP; ++j) {
+            uint32_t v4[4] = {vf[j][i].x, vf[j][i].y, vf[j][i].z, vf[j][i].w};
+            if (CUT) {                                  // positions that are not seen may hold anything
+              const int k0 = h0 + 4 * SPAN * j + SPAN * quad;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                if (F32) v4[w] = (k0 + w >= first && k0 + w <= last) ? v4[w] : 0u;
+                else {
+                  const int ka = k0 + 2 * w;
+                  v4[w] &= ((ka >= first && ka <= last) ? 0x0000ffffu : 0u) | ((ka + 1 >= first && ka + 1 <= last) ? 0xffff0000u : 0u);
+                }
+              }
+            }
+            if (F32) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v4[x]), e[j][x], o, 0, 0, 0);
+            } else {
+              const uint4 v = make_uint4(v4[0], v4[1], v4[2], v4[3]);
+              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, hi[j]), o, 0, 0, 0);
+              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, lw[j]), o, 0, 0, 0);
+            }
+          }
+          // (a column that takes no part keeps its sums: zero times another beam's infinite value is no number)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[y][i][x] = !CUT || takes ? o[x] : acc[y][i][x];
+        }
       }
     };
     auto all_steps = [&](auto cut_tag) {
@@ -304,18 +321,23 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
   }
 
   // ---- the wavefronts' results joined
-  l += __shfl_xor(l, 16, DA_WAVE);
-  l += __shfl_xor(l, 32, DA_WAVE);
-  if (quad == 0) {
-    m_lds[wave][col] = len > 0 ? m : -INFINITY;         // (a place without a beam went along in the shared chunks)
-    l_lds[wave][col] = len > 0 ? l : 0.f;
+#pragma unroll
+  for (int y = 0; y < RT; ++y) {
+    l[y] += __shfl_xor(l[y], 16, DA_WAVE);
+    l[y] += __shfl_xor(l[y], 32, DA_WAVE);
+    const int row = TILE * y + col;
+    if (quad == 0) {
+      m_lds[wave][row] = len[y] > 0 ? m[y] : -INFINITY; // (a place without a beam went along in the shared chunks)
+      l_lds[wave][row] = len[y] > 0 ? l[y] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < DV; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc_lds[wave][16 * i + 4 * quad + x][row] = len[y] > 0 ? acc[y][i][x] : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < DV; ++i)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) acc_lds[wave][16 * i + 4 * quad + x][col] = len > 0 ? acc[i][x] : 0.f;
   __syncthreads();
-  // 16 threads a row, 16 dimensions that follow each other
+  // 16 threads a row, 16 dimensions that follow each other (WAVES / 4 / RT rounds of all rows)
+  static_assert(WAVES * DA_WAVE % (16 * ROWS) == 0, "whole rounds");
   const int row = t / 16 % ROWS, of_row = r0 + row;
   if (of_row >= R) return;
   float w[WAVES], mm = -INFINITY, ll = 0.f;
@@ -358,20 +380,26 @@ attn_beams_merge_kernel(const float* __restrict__ partial, int splits, int pairs
   const float* p = partial + (size_t)pair * splits * (D + 2);
   const float* mine = p + (size_t)(lane < splits ? lane : 0) * (D + 2) + D;
   const float m = lane < splits ? mine[0] : -INFINITY, l = lane < splits ? mine[1] : 0.f;
+  auto load = [&](float v[8], int d0, int z0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p[(size_t)min(z0 + u, splits - 1) * (D + 2) + min(d0 + lane, D - 1)];
+  };
+  float v[8];
+  load(v, 0, 0);                                        // (the first of them travel beside the maxima)
   const float mm = wave_max(m), m_use = mm == -INFINITY ? 0.f : mm;
   const float w = lane < splits ? exp_of_2(m - m_use) : 0.f;
   const float ll = wave_sum(w * l), inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
   for (int d0 = 0; d0 < D; d0 += DA_WAVE) {
-    const int d = d0 + lane;
     float o = 0.f;
     for (int z0 = 0; z0 < splits; z0 += 8) {
-      float v[8];
+      if (d0 + z0 > 0) load(v, d0, z0);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = p[(size_t)min(z0 + u, splits - 1) * (D + 2) + (d < D ? d : 0)];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) o += (z0 + u < splits ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(z0 + u, DA_WAVE - 1))) : 0.f) * v[u];
+      for (int u = 0; u < 8; ++u) {
+        const float wz = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(z0 + u, DA_WAVE - 1)));
+        o += z0 + u < splits ? wz * v[u] : 0.f;
+      }
     }
-    if (d < D) from_f32(out + (size_t)s * out_ld + (size_t)h * D + d, o * inv);
+    if (d0 + lane < D) from_f32(out + (size_t)s * out_ld + (size_t)h * D + d0 + lane, o * inv);
   }
 }
 
@@ -379,10 +407,18 @@ extern "C" int da_attn_beams_takes(int D, int page) {
   return D % 16 == 0 && D >= 16 && D <= BEAMS_MAX_D && page >= 16 && (page & (page - 1)) == 0;
 }
 
+// Rows of a workgroup.  Two tiles where with one there would be more than a workgroup a compute unit, all of which read what they share: 10 x 5 beams,
+// 68 / 17 heads of 64, 853 positions 21.4 us for 27.7, 7 x 7 beams, 95 / 19 heads, 1,956 positions 40.4 for 49.4; with fewer workgroups the
+// second tile's arithmetic is what is waited for (13 x 4 beams, 15 / 3 heads of 80, 3,365 positions 29.8 for 24.8).  Above 64 the registers do not hold it.
+static long beam_groups(int G, int B, int Hq, int Hkv, int rows) { return (long)G * Hkv * da_ceil_div((long)B * (Hq / Hkv), rows); }
+static int beam_rows(int G, int B, int Hq, int Hkv, int D) {
+  return (long)B * (Hq / Hkv) > TILE && D <= 64 && beam_groups(G, B, Hq, Hkv, TILE) > 256 ? 2 * TILE : TILE;
+}
+
 // How many workgroups share a group's positions: from the step's shape only.
 extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int max_blocks, int page) {
   if (G <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_blocks <= 0 || page <= 0) return 1;
-  const long groups = (long)G * Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS);
+  const long groups = beam_groups(G, B, Hq, Hkv, beam_rows(G, B, Hq, Hkv, D));
   const long chunks = ((long)max_blocks * page + CHUNK - 1) / CHUNK;
   // one workgroup a compute unit; a second kernel does not pay for short sequences
   long n = chunks < 8 ? 1 : 256 / groups;
@@ -393,8 +429,7 @@ extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int ma
 // Wavefronts of a workgroup.  8 where there is one workgroup a compute unit, which they fill by themselves: 8 x 8 beams of 25 heads over 1,003 positions
 // 17.3 us for 20.1, 24 beams of 7 heads over 3,456 11.5 for 13.6.  4 where more share one, and where each has so many chunks that 4 wavefronts
 // keep the memory busy: 4 x 4 beams over 32,701 positions, 64 chunks each, 104 us for 113 (26 chunks each: 29.2 for 27.5).
-static int beam_waves(int G, int B, int Hq, int Hkv, int splits, int max_blocks, int page) {
-  const long groups = (long)G * Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS);
+static int beam_waves(long groups, int splits, int max_blocks, int page) {
   return groups * splits > 256 || (long)max_blocks * page / CHUNK >= 48L * splits ? 4 : 8;
 }
 
@@ -402,16 +437,25 @@ template <typename T, int DK, int STEP>
 static void beams_launch(hipStream_t s, const void* q, int q_ld, const void* cache, const int* block_table, int max_blocks, const int* seq_lens,
                          const int* shared, int G, int B, int Hq, int Hkv, int D, int page, float scale, int window, void* out, int out_ld,
                          int splits, float* partial) {
-  const dim3 grid(Hkv * da_ceil_div((long)B * (Hq / Hkv), ROWS), G, splits);
-  if constexpr (DK < 8) {                               // (head sizes above 128 have registers for 4 wavefronts only)
-    if (beam_waves(G, B, Hq, Hkv, splits, max_blocks, page) == 8) {
-      hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP, 8>), grid, dim3(8 * DA_WAVE), 0, s, (const T*)q, q_ld, (const T*)cache, block_table,
-                         max_blocks, seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits, partial);
-      return;
+  const int rows = beam_rows(G, B, Hq, Hkv, D);
+  const dim3 grid(Hkv * da_ceil_div((long)B * (Hq / Hkv), rows), G, splits);
+  const int waves = beam_waves(beam_groups(G, B, Hq, Hkv, rows), splits, max_blocks, page);
+#define DA_BEAMS_AS(WAVES, RT) \
+  hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP, WAVES, RT>), grid, dim3(WAVES * DA_WAVE), 0, s, (const T*)q, q_ld, (const T*)cache, block_table, \
+                     max_blocks, seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits, partial)
+  if constexpr (DK == 8) {                              // (registers for 4 wavefronts only)
+    DA_BEAMS_AS(4, 1);
+  } else {
+    if constexpr (DK <= 2) {
+      if (rows > TILE) {
+        DA_BEAMS_AS(8, 2);
+        return;
+      }
     }
+    if (waves == 8) DA_BEAMS_AS(8, 1);
+    else DA_BEAMS_AS(4, 1);
   }
-  hipLaunchKernelGGL((attn_beams_kernel<T, DK, STEP, 4>), grid, dim3(4 * DA_WAVE), 0, s, (const T*)q, q_ld, (const T*)cache, block_table, max_blocks,
-                     seq_lens, shared, B, Hq, Hkv, D, page, scale, window, (T*)out, out_ld, splits, partial);
+#undef DA_BEAMS_AS
 }
 
 extern "C" int da_attn_beams(const void* q, int q_ld, const void* cache, int dtype, const int* block_table, int max_blocks, const int* seq_lens,

@@ -251,14 +251,17 @@ def _dev(*ts):
 
 def _dev_here(*ts):
     """``_dev``, and on the device whose current stream the launch goes to."""
-    _dev(*ts)
     here = -1
     for t in ts:
-        if t is not None and t.is_cuda:
-            if here < 0:
-                here = torch._C._cuda_getDevice()
-            if t.get_device() != here:
-                raise KernelError(f"kernel operands lie on {t.device}, the current device is cuda:{here}")
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0:
+            _dev(t)
+        elif d != here:
+            if here >= 0 or d != torch._C._cuda_getDevice():
+                raise KernelError(f"kernel operands lie on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+            here = d
 
 
 def _rows_2d(t: torch.Tensor, name: str):

@@ -300,6 +300,8 @@ ATTEND = [  # groups, beams, heads, kv heads, head size, page, lengths, shared
     (1, 16, 2, 2, 64, 16, [1100 + i for i in range(16)], [0]),
     (1, 64, 2, 1, 32, 16, [210] * 64, [192]),
     (1, 2, 1, 1, 64, 16, [5000, 4999], [4096]),
+    (9, 5, 60, 15, 32, 16, [40 + i % 7 for i in range(45)], [32] * 9),       # more workgroups than compute units: two tiles of rows a workgroup
+    (13, 9, 40, 20, 48, 32, [97 if i % 9 else 0 for i in range(117)], [64] * 13),
 ]
 
 
