@@ -49,6 +49,9 @@ def cmd_generate(a) -> int:
         return 2
     if a.max_cases is not None:
         prompts = prompts[:a.max_cases]
+    if a.num_beams is not None and (a.temperature or any(v is not None for v in (a.top_k, a.top_p, a.uniform_top_p, a.xtc_threshold, a.xtc_probability))):
+        print("--num-beams searches for the most likely tokens: it takes no temperature and no filters", file=sys.stderr)
+        return 2
     cfg = {}
     if a.model_config:
         with open(a.model_config) as f:

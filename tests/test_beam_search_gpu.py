@@ -103,6 +103,29 @@ def test_beam_search_in_bfloat16_scores_its_own_tokens(models):
         assert abs(h.score - log_probability(logits_of, prompt, h.tokens)) <= near
 
 
+@pytest.mark.parametrize("dtype,graphs,page", [("float32", True, 16), ("float32", False, 32), ("bfloat16", True, 64)])
+def test_long_prompts_read_what_beams_share_once(dtype, graphs, page, tmp_path, monkeypatch):
+    import helpers
+    import plain_gpt2 as P
+    from deliverance_amd import BeamParameters
+    from deliverance_amd.kernels import ops
+    m = helpers.make_model(tmp_path, dict(helpers.CONFIG_A, n_positions=2048), seed=5)
+    calls = []
+    kernel = ops.attention_beams
+    monkeypatch.setattr(ops, "attention_beams", lambda *a, **k: (calls.append(1), kernel(*a, **k))[1])
+    eng = load(m.folder, dtype, use_graphs=graphs, max_cached_tokens=8192, page_size=page)
+    prompts = [m.prompt(n) for n in (530, 547)]
+    outs = eng.beam_search(prompts, BeamParameters(num_beams=3, max_tokens=9))
+    assert calls
+    logits_of = lambda ids: P.forward_logits(m.plain_cfg, m.W, ids)[-1]  # noqa: E731
+    for prompt, out in zip(prompts, outs):
+        if dtype == "float32":
+            check(out, logits_of, prompt, 3, 9, (511,))
+        else:
+            near = 9 * 2 * 0.04 * float(np.sqrt((logits_of(prompt) ** 2).mean()))
+            assert all(abs(h.score - log_probability(logits_of, prompt, h.tokens)) <= near for h in out.hypotheses)
+
+
 def test_prompts_wait_for_pages_and_places(models):
     import plain_gpt2 as P
     from deliverance_amd import BeamParameters

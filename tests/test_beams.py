@@ -209,3 +209,30 @@ def test_shared_scores_and_positions_of_a_padded_step():
     words = StepRunner._beam_words(BeamStep(2, 4, [-1.5, -math.inf], [[32], [16]]), 2)
     assert np.array(words[:4], dtype=np.int32).view(np.float32).tolist() == [-1.5, -math.inf, -math.inf, -math.inf]
     assert words[4:] == [32, 0, 16, 0]
+
+
+def test_the_command_line_takes_beams_or_sampling():
+    from deliverance_amd import cli
+    for more in (["--temperature", "0.5"], ["--top-k", "4"], ["--top-p", "0.5"], ["--xtc-threshold", "0.1"]):
+        assert cli.main(["generate", "--model", "/nonexistent", "--prompt-ids", "1,2", "--num-beams", "2", *more]) == 2
+
+
+def test_operands_on_another_device_are_refused(monkeypatch):
+    import torch
+    from deliverance_amd.kernels import ops
+
+    class Operand:
+        def __init__(self, index):
+            self.index, self.is_cuda, self.device = index, index >= 0, f"cuda:{index}"
+
+        def get_device(self):
+            return self.index
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    ops._dev_here(Operand(1), None, Operand(1))
+    for bad in ((Operand(0),), (Operand(1), Operand(0)), (Operand(0), Operand(1))):
+        with pytest.raises(ops.KernelError, match="current device is cuda:1"):
+            ops._dev_here(*bad)
+    with pytest.raises(ops.KernelError, match="on the GPU"):
+        ops._dev_here(Operand(1), Operand(-1))

@@ -126,6 +126,20 @@ def test_a_large_score_does_not_make_neighbouring_logits_equal():
     check_select(logits.to(DEV), scores.to(DEV), 2, 30)
 
 
+def test_a_choice_among_more_segments_and_entries_than_the_lists_hold():
+    """Segments in stripes, so that the groups in front are better than the others with everything they have, and entries that are all
+    near their segment's best: the bounds are searched bit by bit."""
+    V = 262144
+    v = torch.arange(V)
+    row = -(v // 256 % 256).double() - (v % 256).double() * 2.0 ** -10
+    logits = torch.stack([row, row]).float()
+    check_select(logits.to(DEV), torch.tensor([-1.0, -1.30078125], device=DEV), 2, 128)
+    # 128 best entries in each of many segments
+    flat = torch.zeros(2, V)
+    flat[:, 1000:200000] = 3.0
+    check_select(flat.to(DEV), torch.tensor([-1.0, -1.0], device=DEV), 2, 128)
+
+
 def test_refusals_of_the_choice():
     logits, scores = torch.zeros(6, 40, device=DEV), torch.zeros(6, device=DEV)
     out = (torch.zeros(2, 4, device=DEV), torch.zeros(2, 4, dtype=torch.int32, device=DEV), torch.zeros(2, 4, dtype=torch.int32, device=DEV))
@@ -368,3 +382,108 @@ def test_refusals_of_attention():
                 dict(q=c["q"][:, :32], out=out[:, :32], n_heads=4, cache_slot=c["cache"][..., :8].contiguous())):
         with pytest.raises(KernelError):
             ops.attention_beams(**{**good, **bad})
+
+
+# ------------------------------------------------------------------------------- as programs use them
+def recorded(f):
+    """``f`` once eagerly, then recorded; a function that replays it."""
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f()
+    return graph.replay
+
+
+@pytest.mark.needs_device
+def test_recorded_calls_follow_their_inputs():
+    """Two recordings that share a workspace, replayed in turn with other work between them, on inputs that change."""
+    g = torch.Generator().manual_seed(31)
+    logits, scores = torch.randn(8, 3001, device=DEV), -torch.rand(8, device=DEV)
+    out = (torch.zeros(2, 8, device=DEV), torch.zeros(2, 8, dtype=torch.int32, device=DEV), torch.zeros(2, 8, dtype=torch.int32, device=DEV))
+    c = beams_case(2, 4, 4, 4, 64, 16, torch.bfloat16, [700] * 8, [640, 656], seed=4)
+    D, splits = 64, 3
+    o = torch.zeros(8, 256, dtype=torch.bfloat16, device=DEV)
+    ws = torch.zeros(max(ops.beam_select_floats(8, 4, 3001), ops.beam_workspace_floats(8, 4, D, splits)), device=DEV)
+    state = torch.randn(12, 1000, device=DEV)
+    slots = torch.tensor([[3, 1, 7, 0], [2, 11, 5, 6]], dtype=torch.int32, device=DEV)
+    parents = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+
+    def choose():
+        ops.beam_select(logits, scores, 4, *out, ws)
+
+    def rest():
+        ops.attention_beams(c["q"], c["cache"], c["table"], c["lens"], c["shared"], 4, 4, 0.125, None, o, splits, ws)
+        ops.state_reorder([state], slots, parents)
+
+    first, second = recorded(choose), recorded(rest)
+    for turn in range(4):
+        logits.copy_(torch.randn(8, 3001, generator=g) * 2)
+        scores.copy_(-torch.rand(8, generator=g) * 5)
+        c["q"].copy_(torch.randn(8, 256, generator=g).bfloat16())
+        state.copy_(torch.randn(12, 1000, generator=g))
+        parents.copy_(torch.randint(0, 4, (2, 4), generator=g))
+        first()
+        want_state = plain_reorder([state.cpu()], slots.cpu(), parents.cpu(), 0)[0]
+        second()
+        want = plain_select(logits, scores, 4, 8)
+        assert torch.equal(out[1].cpu().long(), want[1]) and torch.equal(out[2].cpu().long(), want[2])
+        assert torch.equal(state.cpu(), want_state)
+        eager = torch.zeros_like(o)
+        ops.attention_beams(c["q"], c["cache"], c["table"], c["lens"], c["shared"], 4, 4, 0.125, None, eager, splits, torch.zeros_like(ws))
+        assert torch.equal(eager, o)
+        near = 2.0 ** -8 * plain_attention(c).abs() + 1.2e-3
+        assert bool(((o.cpu().double() - plain_attention(c)).abs() <= near).all())
+
+
+@pytest.mark.needs_device
+def test_a_chain_of_steps_on_a_stream_of_its_own():
+    """The three operators together, as a step uses them: attention, a choice, and what is kept follows it, all without the host."""
+    stream = torch.cuda.Stream()
+    g = torch.Generator().manual_seed(8)
+    G, B, D, V = 2, 3, 32, 500
+    c = beams_case(G, B, 2, 2, D, 16, torch.float32, [200] * 6, [192] * 2, seed=2)
+    head = torch.randn(2 * D, V, generator=g)
+    state = torch.randn(10, 77, generator=g)
+    slots = torch.tensor([[9, 2, 4], [0, 7, 3]], dtype=torch.int32)
+    scores = -torch.rand(G * B, generator=g)
+    o = plain_attention(c)
+    want = plain_select((o.float() @ head), scores, B, B)
+    want_state = plain_reorder([state], slots, want[1].int(), 0)[0]
+    dev = [t.to(DEV) for t in (head, state, slots, scores)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        got = attend(c, splits=2)
+        logits = got @ dev[0]
+        out = (torch.empty(G, B, device=DEV), torch.empty(G, B, dtype=torch.int32, device=DEV), torch.empty(G, B, dtype=torch.int32, device=DEV))
+        ops.beam_select(logits, dev[3], B, *out, torch.empty(ops.beam_select_floats(G * B, B, V), device=DEV))
+        ops.state_reorder([dev[1]], dev[2], out[1])
+    stream.synchronize()
+    assert float(want[3].min()) > 1e-4                      # (32-bit logits of this size are off by about 1e-5)
+    assert torch.equal(out[1].cpu().long(), want[1]) and torch.equal(out[2].cpu().long(), want[2])
+    assert torch.equal(dev[1].cpu(), want_state)
+
+
+@pytest.mark.needs_device
+def test_places_beyond_32_bits():
+    """A cache, states and logits whose last rows lie more than 2^32 bytes behind the first ones."""
+    Hkv, page, D, n = 8, 64, 128, 24000                      # 6.3 GB
+    big = torch.empty(n, 2, Hkv, page, D, dtype=torch.bfloat16, device=DEV)
+    c = beams_case(1, 2, 8, Hkv, D, page, torch.bfloat16, [150, 140], [128], seed=3)
+    few = c["cache"].shape[0]
+    big[n - few:] = c["cache"]
+    far = dict(c, cache=big, table=torch.where(c["table"] >= 0, c["table"] + (n - few), -1).int())
+    assert torch.equal(attend(far), attend(c))
+    del big, far
+    row = 1 << 28                                            # 1 GiB a row
+    t = torch.empty(6, row, dtype=torch.float32, device=DEV)
+    for i in range(6):
+        t[i, -3:] = i
+        t[i, :3] = 10 + i
+    ops.state_reorder([t], torch.tensor([[5, 0, 4]], dtype=torch.int32, device=DEV), torch.tensor([[1, 0, 0]], dtype=torch.int32, device=DEV))
+    assert t[:, -1].tolist() == [5, 1, 2, 3, 5, 0] and t[:, 0].tolist() == [15, 11, 12, 13, 15, 10]
+    del t
+    wide = torch.empty(6, 1 << 29, dtype=torch.float32, device=DEV)
+    part = wide[:, 7:1007]
+    part.copy_(torch.randn(6, 1000, generator=torch.Generator().manual_seed(9)))
+    check_select(part, torch.tensor([-1.0, -1.5, -2.5] * 2, device=DEV), 3, 6)
