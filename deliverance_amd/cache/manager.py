@@ -319,7 +319,8 @@ class CacheManager:
             new = [t if p == i else old[p][:full] + t[full:] for i, (t, p) in enumerate(zip(old, parents))]
             for rid, before, after in zip(rids, old, new):        # everybody takes before anybody gives
                 if after is not before:
-                    pool.share([p for p in after[:full] if p >= 0 and not pool.held_by(p, rid)], rid)
+                    have = set(before)
+                    pool.share([p for p in after[:full] if p >= 0 and p not in have], rid)
             for rid, r, before, after in zip(rids, reqs, old, new):
                 if after is not before:
                     r.tables[g] = after

@@ -8,7 +8,7 @@
 // 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  The terms of the sum are 32-bit exponentials,
 // summed in 64-bit.
 //
-// Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 512 or 2,048 logits of a row and leaves their maximum
+// Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 512 or 1,024 logits of a row and leaves their maximum
 // and sum, and the largest of each segment of 64 or 256.  beam_choose_kernel, one workgroup a group, works on what is left, by a bound
 // that K entries surely reach: the best segments of n groups of segments are n entries, and the K-th best of them is such a bound (about K + K^2 / 2n
 // segments reach it).  It reads the segments that reach it again; the entries that do are cut down by bounds of the same
@@ -20,7 +20,7 @@
 #define BEAM_MAX_KEEP 128        // candidates of a group
 #define LOAD 256                 // logits of a wavefront's load: 64 lanes, 4 each
 #define LOADS_FEW 2              // of a wavefront: few logits, or many
-#define LOADS_MANY 8
+#define LOADS_MANY 4
 #define STATS_WAVES 4
 #define CHOOSE_THREADS 1024
 #define CHOOSE_WAVES (CHOOSE_THREADS / DA_WAVE)
@@ -61,7 +61,7 @@ beam_stats_kernel(const float* __restrict__ logits, long ldl, int V, int n_segs,
   if (v0 + LOADS * LOAD <= V) {
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) {
-      const float4_any f = *(const float4_any*)(z + v0 + s * LOAD + 4 * lane);
+      const float4_any f = __builtin_nontemporal_load((const float4_any*)(z + v0 + s * LOAD + 4 * lane));
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[s][e] = f[e];
     }
@@ -410,7 +410,7 @@ struct Cut {
 static Cut beam_cut(long rows, int B, int V) {
   Cut c;
   c.seg = (long)B * (((long)V + 63) / 64) <= HELD * CHOOSE_THREADS ? 64 : 256;
-  c.loads = rows * (((long)V + LOAD - 1) / LOAD) < 8192 ? LOADS_FEW : LOADS_MANY;
+  c.loads = rows * (((long)V + LOAD - 1) / LOAD) < 16384 ? LOADS_FEW : LOADS_MANY;
   c.n_segs = ((long)V + c.seg - 1) / c.seg;
   c.n_parts = ((long)V + c.loads * LOAD - 1) / (c.loads * LOAD);
   return c;

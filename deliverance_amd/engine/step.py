@@ -220,7 +220,8 @@ class StepRunner:
         sequences only, the step and its sampling are replayed from a recorded HIP graph and the
         sampled tokens are left in ``ctx.sampled`` (the first rows of ``self.sampled``).  With ``beams`` (in place of
         ``sample_records``) the step's entries are beams, one token each whose logits are wanted, and the choice of the next ones
-        (``ops.beam_select``) is left in ``ctx.chosen``: scores, parents and tokens, [requests, n_keep] each, on the device."""
+        (``ops.beam_select``) is left in ``ctx.chosen``, int32 [3, requests, n_keep] on the device: the bits of the 32-bit scores, parents
+        and tokens."""
         mgr = self.cache.manager
         cfg = self.model.config
         if not entries:
@@ -332,10 +333,10 @@ class StepRunner:
     def _choose(self, ctx, beams: BeamStep, logits: torch.Tensor):
         from ..kernels import ops
         per = ctx.n_seqs // beams.n_beams
-        out = (ctx.buf("beam_out_scores", per, beams.n_keep, torch.float32), ctx.buf("beam_out_parents", per, beams.n_keep, torch.int32),
-               ctx.buf("beam_out_tokens", per, beams.n_keep, torch.int32))
+        chosen = ctx.flat("beam_chosen", 3 * per * beams.n_keep, torch.int32).view(3, per, beams.n_keep)
         ws = ctx.flat("beam_select", ops.beam_select_floats(logits.shape[0], beams.n_beams, logits.shape[1]), torch.float32)
-        return ops.beam_select(logits, ctx.beam_scores, beams.n_beams, *out, ws)
+        ops.beam_select(logits, ctx.beam_scores, beams.n_beams, chosen[0].view(torch.float32), chosen[1], chosen[2], ws)
+        return chosen
 
     def _run_eager(self, entries, order, starts, sample_records, beams=None):
         from ..kernels import ops
@@ -453,5 +454,5 @@ class StepRunner:
         if beams is None:
             ctx.sampled = sampled[:S]
         else:
-            ctx.chosen = tuple(t[:S // unit] for t in st["chosen"])
+            ctx.chosen = st["chosen"][:, :S // unit]
         return st["logits"][:S], ctx

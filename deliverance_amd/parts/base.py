@@ -124,6 +124,7 @@ class StepContext:
         self.beam_shared: List[torch.Tensor] = []
         self.beam_shared_host: List[List[int]] = []
         self.beam_scores: torch.Tensor = None
+        self.chosen: torch.Tensor = None               # int32 [3, S / n_beams, candidates], what the step's choice left (engine/step.py)
         self.cache = None                              # engine.DeviceCache
         self._arena = None
         # False while a part runs that was given a buffer of its own to fill (a norm follows it): a part
