@@ -5,8 +5,8 @@
 //
 // A logit that is -inf or no number is never chosen and adds nothing to the sum; a score that is -inf or no number marks a
 // place without a beam; where the largest logit is infinite, the entries that reach it share the probability.  Keys are 64-bit: a
-// 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  The terms of the sum are 32-bit exponentials,
-// summed in 64-bit.
+// 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  The terms of the sum are 32-bit exponentials;
+// four that lie side by side are added in 32-bit (two roundings of 2^-24), the rest in 64-bit.
 //
 // Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 512 or 1,024 logits of a row and leaves their maximum
 // and sum, and the largest of each segment of 64 or 256.  beam_choose_kernel, one workgroup a group, works on what is left, by a bound
@@ -24,7 +24,8 @@
 #define STATS_WAVES 4
 #define CHOOSE_THREADS 1024
 #define CHOOSE_WAVES (CHOOSE_THREADS / DA_WAVE)
-#define HELD 2                   // segments whose keys a thread, and whose entries a wavefront keeps
+#define SHORT_SEGS 2048          // segments of a group up to which they are short
+#define SIDES_HELD 2             // loads of segments' entries whose keys a wavefront keeps
 #define SEG_LIST 512             // segments that are read again
 #define LIST 4096                // their entries that reach the bound
 #define LIST_A_THREAD (LIST / CHOOSE_THREADS)
@@ -187,7 +188,8 @@ __device__ void narrow(Chosen& bound, uint64_t largest, int keep, int most, Coun
 }
 
 // magic: 2^32 / n_segs rounded up (0: divide), for fewer than 65,536 segments
-template <int SEG>
+// HELD: segments whose keys a thread keeps (those behind them it works out again)
+template <int SEG, int HELD>
 __global__ void __launch_bounds__(CHOOSE_THREADS)
 beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int K, const float* __restrict__ scores, int n_segs,
                    int n_parts, const float* __restrict__ seg_max, const float* __restrict__ part_max, const double* __restrict__ part_sum,
@@ -314,10 +316,10 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     return b * V + v;
   };
   const int n_sides = (n_found + SIDE - 1) / SIDE;
-  uint64_t kept[HELD][4];
-  int place_kept[HELD];
+  uint64_t kept[SIDES_HELD][4];
+  int place_kept[SIDES_HELD];
 #pragma unroll
-  for (int h = 0; h < HELD; ++h) {
+  for (int h = 0; h < SIDES_HELD; ++h) {
     place_kept[h] = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) kept[h][e] = 0;
@@ -325,10 +327,10 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
   }
   auto each_entry = [&](auto f) {
 #pragma unroll
-    for (int h = 0; h < HELD; ++h)
+    for (int h = 0; h < SIDES_HELD; ++h)
 #pragma unroll
       for (int e = 0; e < 4; ++e) f(kept[h][e], place_kept[h] + e);
-    for (int j = wave + HELD * CHOOSE_WAVES; j < n_sides; j += CHOOSE_WAVES) {
+    for (int j = wave + SIDES_HELD * CHOOSE_WAVES; j < n_sides; j += CHOOSE_WAVES) {
       uint64_t k[4];
       const int place = keys_of(j, k);
 #pragma unroll
@@ -409,7 +411,7 @@ struct Cut {
 };
 static Cut beam_cut(long rows, int B, int V) {
   Cut c;
-  c.seg = (long)B * (((long)V + 63) / 64) <= HELD * CHOOSE_THREADS ? 64 : 256;
+  c.seg = (long)B * (((long)V + 63) / 64) <= SHORT_SEGS ? 64 : 256;
   c.loads = rows * (((long)V + LOAD - 1) / LOAD) < 16384 ? LOADS_FEW : LOADS_MANY;
   c.n_segs = ((long)V + c.seg - 1) / c.seg;
   c.n_parts = ((long)V + c.loads * LOAD - 1) / (c.loads * LOAD);
@@ -450,11 +452,12 @@ extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V
   DA_CHECK_LAUNCH("beam_select (sums)");
   // i * magic / 2^32 is i / n_segs while i < 2^16 and n_segs < 2^16: the product's error, i * (magic * n_segs - 2^32) / n_segs / 2^32, is below i / 2^32
   const uint32_t magic = (long)B * n_segs < 65536 && n_segs > 1 ? (uint32_t)(((1ull << 32) + n_segs - 1) / n_segs) : 0;
-#define DA_CHOOSE(SEG) \
-  hipLaunchKernelGGL((beam_choose_kernel<SEG>), dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts, \
+#define DA_CHOOSE(SEG, HELD) \
+  hipLaunchKernelGGL((beam_choose_kernel<SEG, HELD>), dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts, \
                      seg_max, part_max, part_sum, out_score, out_parent, out_token, magic)
-  if (cut.seg == 64) DA_CHOOSE(64);
-  else DA_CHOOSE(256);
+  if (cut.seg == 64) DA_CHOOSE(64, 2);
+  else if (B * n_segs <= 2 * CHOOSE_THREADS) DA_CHOOSE(256, 2);
+  else DA_CHOOSE(256, 4);                               // (32 x 8 beams, 131,071: 34.4 us for 37.1)
 #undef DA_CHOOSE
   DA_CHECK_LAUNCH("beam_select (choice)");
   return 0;

@@ -48,9 +48,9 @@ def select(logits, scores, B, K):
 
 def check_select(logits, scores, B, K):
     want = plain_select(logits, scores, B, K)
-    # The kernel's sum of exponentials is off by the 32-bit exponential (two units in its last place: 2^-22) and the operand's
-    # rounding (2^-24 of a difference below 90, weighed with its term e^-difference: below 2^-24); so keys of two beams compare as the
-    # 64-bit ones do where they are 1e-6 apart, or equal.
+    # The kernel's sum of exponentials is off by the 32-bit exponentials (two units in the last place: 2^-22), by the two roundings that add
+    # four of them (2^-23) and by the operands' rounding (2^-24 of a difference d, weighed with its term e^-d: below 2^-24), together below
+    # 2^-21; so keys of two beams compare as the 64-bit ones do where they are 1e-6 apart, or equal.
     gaps = want[3]
     assert bool(((gaps == 0.0) | (gaps > 1e-6)).all()), "the inputs do not keep the keys apart"
     got = select(logits, scores, B, K)
