@@ -415,13 +415,14 @@ static int beam_rows(int G, int B, int Hq, int Hkv, int D) {
   return (long)B * (Hq / Hkv) > TILE && D <= 64 && beam_groups(G, B, Hq, Hkv, TILE) > 256 ? 2 * TILE : TILE;
 }
 
-// How many workgroups share a group's positions: from the step's shape only.
-extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int max_blocks, int page) {
+// How many workgroups share a group's positions: from the step's shape only.  One workgroup a compute unit; a second kernel, which joins the shares,
+// does not pay for few chunks (bfloat16, 1 x 4 beams of 12 heads of 64, 9 chunks: 7.7 us with one workgroup, 8.1 with four, and a launch more on the
+// host; 16 chunks 9.8 and 8.0; heads of 128, 11 chunks 13.8 and 10.3).  In 32-bit, whose products take 16 times as long, it does: 2 x 5 beams, 9 chunks 19.3 and 11.8.
+extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int dtype, int max_blocks, int page) {
   if (G <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_blocks <= 0 || page <= 0) return 1;
   const long groups = beam_groups(G, B, Hq, Hkv, beam_rows(G, B, Hq, Hkv, D));
   const long chunks = ((long)max_blocks * page + CHUNK - 1) / CHUNK;
-  // one workgroup a compute unit; a second kernel does not pay for short sequences
-  long n = chunks < 8 ? 1 : 256 / groups;
+  long n = chunks < (dtype == DA_F32 ? 4 : (D <= 64 ? 12 : 8)) ? 1 : 256 / groups;
   if (n > chunks / 2) n = chunks / 2;
   return n < 1 ? 1 : (n > DA_WAVE ? DA_WAVE : (int)n);
 }

@@ -76,17 +76,19 @@ reorder_kernel(const ReorderTable table, const int* __restrict__ slots, const in
   }
 }
 
-// n tensors [layers, pool, row]; `data`, `row_bytes` (even) and `layers` are host arrays.
-extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const int* layers, int n, int pool, const int* slots,
-                                const int* parents, int G, int B, void* stream) {
+// n tensors [layers, pool, row]: a host array of three numbers each, their address, their row's bytes (even) and layers.
+extern "C" int da_state_reorder(const long* tensors, int n, int pool, const int* slots, const int* parents, int G, int B, void* stream) {
+  auto data = [&](int i) { return (char*)tensors[3 * i]; };
+  auto row_bytes = [&](int i) { return tensors[3 * i + 1]; };
+  auto layers = [&](int i) { return tensors[3 * i + 2]; };
   DA_REQUIRE(n >= 0 && G >= 0 && G <= 65535 && B > 0 && B <= REORDER_MAX && pool >= 0,
              "state_reorder: bad sizes (tensors=%d rows=%d groups=%d places=%d; at most %d places)", n, pool, G, B, REORDER_MAX);
   for (int i = 0; i < n; ++i)
-    DA_REQUIRE(row_bytes[i] > 0 && row_bytes[i] % 2 == 0 && row_bytes[i] < (1L << 31) && (uintptr_t)data[i] % 2 == 0 && layers[i] >= 0,
-               "state_reorder: %d layers with a row of %ld bytes: not whole 2-byte units, or too long", layers[i], row_bytes[i]);
+    DA_REQUIRE(row_bytes(i) > 0 && row_bytes(i) % 2 == 0 && row_bytes(i) < (1L << 31) && (uintptr_t)data(i) % 2 == 0 && layers(i) >= 0,
+               "state_reorder: %ld layers with a row of %ld bytes: not whole 2-byte units, or too long", layers(i), row_bytes(i));
   if (n == 0 || G == 0 || B == 1 || pool == 0) return 0;
   auto unit_of = [&](int i) {
-    const uintptr_t odd = (uintptr_t)data[i] | (uintptr_t)row_bytes[i];
+    const uintptr_t odd = (uintptr_t)data(i) | (uintptr_t)row_bytes(i);
     return odd % 4 ? 2 : (B <= 16 ? 16 : 4);
   };
   for (int unit = 16; unit > 1; unit = unit == 16 ? 4 : unit - 2) {      // 16, 4, 2
@@ -108,10 +110,10 @@ extern "C" int da_state_reorder(void* const* data, const long* row_bytes, const 
     };
     for (int i = 0; i < n; ++i) {
       if (unit_of(i) != unit) continue;
-      for (int layer = 0; layer < layers[i]; ++layer) {
-        table.data[count] = (char*)data[i] + (long)layer * pool * row_bytes[i];
-        table.bytes[count] = (int)row_bytes[i];
-        const int units = (int)(row_bytes[i] / unit) + (unit == 16 ? (int)(row_bytes[i] % 16 / 4) : 0);
+      for (long layer = 0; layer < layers(i); ++layer) {
+        table.data[count] = data(i) + layer * pool * row_bytes(i);
+        table.bytes[count] = (int)row_bytes(i);
+        const int units = (int)(row_bytes(i) / unit) + (unit == 16 ? (int)(row_bytes(i) % 16 / 4) : 0);
         longest = units > longest ? units : longest;
         if (++count == REORDER_TENSORS) launch();
       }

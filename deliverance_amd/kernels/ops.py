@@ -186,9 +186,9 @@ _ARGTYPES = {
                          _VP, ctypes.c_long, _VP],
     "da_beam_select_words": [_I, _I, _I],
     "da_beam_select": [_VP, ctypes.c_long, _I, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, ctypes.c_long, _VP],
-    "da_state_reorder": [_VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP],
+    "da_state_reorder": [_VP, _I, _I, _VP, _VP, _I, _I, _VP],
     "da_attn_beams_takes": [_I, _I],
-    "da_attn_beams_splits": [_I, _I, _I, _I, _I, _I, _I],
+    "da_attn_beams_splits": [_I, _I, _I, _I, _I, _I, _I, _I],
     "da_attn_beams": [_VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP, _I, _I, _VP, ctypes.c_long, _VP],
 }
 _LIB = None
@@ -375,7 +375,7 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
     if n == 0:
         return tensors
     pool = tensors[0].shape[dim] if tensors[0].dim() > dim else -1
-    ptrs, row_bytes, layers, spans = [], [], [], []
+    table, spans = [], []
     for i, t in enumerate(tensors):
         if t.dim() <= dim or t.shape[dim] != pool or not t.is_contiguous():
             raise KernelError(f"state_reorder: tensor {i} is {list(t.shape)}: contiguous tensors with {pool} rows along dimension {dim} are needed")
@@ -383,9 +383,7 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
         row = size // (pool * k) if size else 2
         if row % 2:
             raise KernelError(f"state_reorder: a row of tensor {i} has {row} bytes, whole 2-byte units are needed")
-        ptrs.append(_ptr(t))
-        row_bytes.append(row)
-        layers.append(k if size else 0)
+        table += (_ptr(t), row, k if size else 0)
         spans.append((t.data_ptr(), size))
     if n > 1:
         spans.sort()
@@ -394,8 +392,9 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
             if a < end and size:
                 raise KernelError("state_reorder: two tensors share memory")
             end = max(end, a + size)
-    with _timed("state_reorder", 2 * G * B * sum(r * k for r, k in zip(row_bytes, layers)) if KernelProfiler.enabled else 0, 0, "fp32"):
-        _check(_lib().da_state_reorder((ctypes.c_void_p * n)(*ptrs), (ctypes.c_long * n)(*row_bytes), (ctypes.c_int * n)(*layers), n, pool, _ptr(slots), _ptr(parents), G, B, _stream()))
+    nbytes = 2 * G * B * sum(table[1::3][i] * table[2::3][i] for i in range(n)) if KernelProfiler.enabled else 0
+    with _timed("state_reorder", nbytes, 0, "fp32"):
+        _check(_lib().da_state_reorder((ctypes.c_long * (3 * n))(*table), n, pool, _ptr(slots), _ptr(parents), G, B, _stream()))
     return tensors
 
 
@@ -1342,10 +1341,11 @@ def attention_beams_takes(head_dim: int, page: int) -> bool:
     return bool(_lib().da_attn_beams_takes(int(head_dim), int(page)))
 
 
-def beam_splits(n_groups: int, n_beams: int, n_heads: int, n_kv_heads: int, head_dim: int, max_blocks: int, page: int) -> int:
+def beam_splits(n_groups: int, n_beams: int, n_heads: int, n_kv_heads: int, head_dim: int, max_blocks: int, page: int,
+                dtype: torch.dtype = torch.bfloat16) -> int:
     """How many workgroups share a group's positions in ``attention_beams`` (1: none do).  The library's rule, from the step's shape
     only, so that a recorded step keeps it."""
-    return int(_lib().da_attn_beams_splits(n_groups, n_beams, n_heads, n_kv_heads, head_dim, max_blocks, page))
+    return int(_lib().da_attn_beams_splits(n_groups, n_beams, n_heads, n_kv_heads, head_dim, F32 if dtype == torch.float32 else BF16, max_blocks, page))
 
 
 def beam_workspace_floats(n_seqs: int, n_heads: int, head_dim: int, n_splits: int) -> int:
@@ -1468,7 +1468,7 @@ def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, 
 
     if (getattr(ctx, "n_beams", 0) > 1 and attention_beams_pays(ctx, group, n_heads, Hkv, D, page) and q.dtype == ctx.dtype and q.stride(0) * el % 16 == 0
             and q.data_ptr() % 16 == 0 and cache_slot.data_ptr() % 16 == 0):
-        n_splits = beam_splits(nd // ctx.n_beams, ctx.n_beams, n_heads, Hkv, D, bt.shape[1], page)
+        n_splits = beam_splits(nd // ctx.n_beams, ctx.n_beams, n_heads, Hkv, D, bt.shape[1], page, q.dtype)
         ws = ctx.flat("beam_partial", beam_workspace_floats(nd, n_heads, D, n_splits), torch.float32) if n_splits > 1 else None
         nbytes, flops = cost(0, nd)                       # (what a group shares is read once)
         again = (ctx.n_beams - 1) * sum(ctx.beam_shared_host[group]) * 2 * Hkv * D * el if nbytes and not window else 0

@@ -324,7 +324,7 @@ ATTEND = [  # groups, beams, heads, kv heads, head size, page, lengths, shared
 def test_attention_of_beams(groups, beams, heads, kv_heads, dim, page, lengths, shared, dtype):
     c = beams_case(groups, beams, heads, kv_heads, dim, page, dtype, lengths, shared, seed=dim + beams, wide=16)
     blocks = c["table"].shape[1]
-    for splits in sorted({1, 3, ops.beam_splits(groups, beams, heads, kv_heads, dim, blocks, page)}):
+    for splits in sorted({1, 3, ops.beam_splits(groups, beams, heads, kv_heads, dim, blocks, page, dtype)}):
         check_attention(c, splits=splits)
 
 
