@@ -7,8 +7,8 @@
 // Rows that stay are neither read nor written.
 //
 // Bound by memory: every row that moves is read and written once.  Loads and stores go past the caches: 8 x 8 beams' pages of 48
-// layers of 25 heads, 315 MB, take 63.5 us (4.96 TB/s, a large copy 5.13) and 98 with ordinary ones, states of 543 MB 112 and
-// 207; several columns a thread are behind (2: 64.9, 117).
+// layers of 25 heads, 315 MB, take 62.9 us (5.0 TB/s, a large copy 5.13) and 98 with ordinary ones, states of 543 MB 112 and
+// 207; two columns a thread are behind (64.9, 117).
 #include "common.h"
 #include <da_anew.h>
 
