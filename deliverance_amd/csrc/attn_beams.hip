@@ -465,7 +465,7 @@ static void beams_launch(hipStream_t s, const void* q, int q_ld, const void* cac
 extern "C" int da_attn_beams(const void* q, int q_ld, const void* cache, int dtype, const int* block_table, int max_blocks, const int* seq_lens,
                              const int* shared, int G, int B, int Hq, int Hkv, int D, int page, float scale, int window, void* out, int out_ld,
                              int splits, float* workspace, long workspace_floats, void* stream) {
-  DA_REQUIRE(G >= 0 && B > 0 && B <= BEAMS_MAX && (long)G * B <= 65535 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && max_blocks > 0 && window >= 0,
+  DA_REQUIRE(G >= 0 && B > 0 && B <= BEAMS_MAX && (long)G * B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 32767 && Hq % Hkv == 0 && max_blocks > 0 && window >= 0,
              "attention_beams: bad sizes (groups=%d beams=%d heads=%d/%d blocks=%d window=%d; at most %d beams)", G, B, Hq, Hkv, max_blocks, window, BEAMS_MAX);
   DA_REQUIRE(da_attn_beams_takes(D, page), "attention_beams: head size %d (multiples of 16 up to %d), page %d (powers of two from 16)", D, BEAMS_MAX_D, page);
   DA_REQUIRE(dtype == DA_F32 || dtype == DA_BF16, "attention_beams: dtype %d", dtype);

@@ -362,7 +362,7 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     n_entries = list_entries();
   }
 
-  // ---- few of them: by bounds of the same kind
+  // ---- few of them: by bounds of the same kind (there are more entries than groups, neighbours in different ones: each group has some)
   while (n_entries > CHOOSE_THREADS / lanes * 3 / 2) {
     Chosen mine[LIST_A_THREAD], first{0, 0x7fffffff};
 #pragma unroll
@@ -430,7 +430,7 @@ extern "C" int da_beam_select_words(int G, int B, int V) {
 
 extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V, const float* scores, int K, float* out_score,
                               int* out_parent, int* out_token, float* scratch, long scratch_words, void* stream) {
-  DA_REQUIRE(G >= 0 && B > 0 && B <= BEAM_MAX && V > 0 && ldl >= V && (long)B * V <= 0x7fffffffL,
+  DA_REQUIRE(G >= 0 && B > 0 && B <= BEAM_MAX && V > 0 && ldl >= V && (long)B * V <= 0x7fff0000L,
              "beam_select: bad sizes (groups=%d beams=%d vocabulary=%d row length %ld; at most %d beams)", G, B, V, ldl, BEAM_MAX);
   DA_REQUIRE(K > 0 && K <= BEAM_MAX_KEEP, "beam_select: %d candidates (1 to %d)", K, BEAM_MAX_KEEP);
   if (G == 0) return 0;

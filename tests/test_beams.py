@@ -236,3 +236,54 @@ def test_operands_on_another_device_are_refused(monkeypatch):
             ops._dev_here(*bad)
     with pytest.raises(ops.KernelError, match="on the GPU"):
         ops._dev_here(Operand(1), Operand(-1))
+
+
+def test_entry_points_refuse_sizes_before_they_launch():
+    """Sizes outside the kernels' limits end with a message, whatever the pointers (no GPU is touched)."""
+    from deliverance_amd.kernels import build, ops
+    try:
+        build.build(only=["beam_select", "reorder", "attn_beams"], verbose=False)
+    except build.KernelLibraryError as e:
+        pytest.skip(str(e))
+    lib = ops._lib()
+
+    def refused(rc, word):
+        assert rc != 0 and word in build.load().da_last_error().decode()
+
+    def select(ldl=50, G=1, B=1, V=50, K=2, scratch=8, words=10 ** 6):
+        return lib.da_beam_select(8, ldl, G, B, V, 8, K, 8, 8, 8, scratch, words, None)
+    for bad in (dict(V=0), dict(ldl=49), dict(B=65), dict(B=0), dict(G=-1), dict(V=2 ** 31 - 1, ldl=2 ** 31), dict(B=64, V=2 ** 26, ldl=2 ** 26)):
+        refused(select(**bad), "bad sizes")
+    refused(select(K=0), "candidates")
+    refused(select(K=129), "candidates")
+    refused(select(G=1025, B=64), "rows")
+    refused(select(scratch=12), "scratch")
+    refused(select(words=3), "scratch")
+    refused(select(scratch=None), "scratch")
+    assert select(G=0) == 0 and lib.da_beam_select_words(-1, 1, 5) == -1 and lib.da_beam_select_words(2 ** 20, 64, 2 ** 20) == -1
+
+    import ctypes
+
+    def reorder(row=8, layers=1, n=1, pool=4, G=1, B=2, at=64):
+        return lib.da_state_reorder((ctypes.c_long * 3)(at, row, layers), n, pool, 8, 8, G, B, None)
+    for bad in (dict(B=0), dict(B=65), dict(G=65536), dict(pool=-1), dict(n=-1)):
+        refused(reorder(**bad), "bad sizes")
+    for bad in (dict(row=3), dict(row=0), dict(row=2 ** 31), dict(at=65), dict(layers=-1)):
+        refused(reorder(**bad), "whole 2-byte units")
+    assert reorder(n=0) == 0 and reorder(G=0) == 0 and reorder(B=1) == 0 and reorder(pool=0) == 0
+
+    def attend(q=16, q_ld=64, cache=16, dtype=ops.BF16, blocks=4, G=1, B=2, Hq=2, Hkv=1, D=32, page=16, window=0, splits=1, ws=None, floats=0):
+        return lib.da_attn_beams(q, q_ld, cache, dtype, 8, blocks, 8, 8, G, B, Hq, Hkv, D, page, 1.0, window, 8, 64, splits, ws, floats, None)
+    for bad in (dict(B=0), dict(B=65), dict(G=-1), dict(G=1025, B=64), dict(Hq=3, Hkv=2), dict(Hq=2 ** 15), dict(Hkv=0), dict(blocks=0), dict(window=-1)):
+        refused(attend(**bad), "bad sizes")
+    for bad in (dict(D=24), dict(D=272), dict(page=8), dict(page=48)):
+        refused(attend(**bad), "head size")
+    refused(attend(dtype=7), "dtype")
+    for bad in (dict(q=8), dict(q_ld=65), dict(cache=8)):
+        refused(attend(**bad), "16 bytes")
+    refused(attend(blocks=2 ** 28), "too large")
+    for n in (0, 65):
+        refused(attend(splits=n), "shares")
+    refused(attend(splits=2), "workspace")
+    refused(attend(splits=2, ws=64, floats=2 * 2 * 2 * 34 - 1), "workspace")
+    assert attend(G=0) == 0
