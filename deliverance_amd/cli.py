@@ -102,11 +102,16 @@ def cmd_generate(a) -> int:
         with open(a.jsonl_output, "w") as f:
             for r in rows:
                 f.write(json.dumps(r) + "\n")
+    _print_profile(a)
+    return 0
+
+
+def _print_profile(a) -> None:
+    from .profiler import InferenceProfiler, KernelProfiler
     if a.profile_stages:
         print(InferenceProfiler.summary("(stages drained at their end)"), file=sys.stderr)
         print(KernelProfiler.summary("(device time per kernel against what it must move and compute; % of 8 TB/s or of "
                                      "the matrix peak, whichever binds)"), file=sys.stderr)
-    return 0
 
 
 def _beam_search(a, model, prompts) -> int:
@@ -114,8 +119,11 @@ def _beam_search(a, model, prompts) -> int:
     from .engine.beams import BeamParameters
     params = BeamParameters(num_beams=a.num_beams, max_tokens=a.max_tokens, ntokens=a.ntokens, length_penalty=a.length_penalty,
                             early_stopping=a.early_stopping, ignore_eos=a.ignore_eos)
+    from .profiler import InferenceProfiler, KernelProfiler
     for p in prompts[:a.warmup_cases]:
         model.beam_search(p, params)
+    InferenceProfiler.reset()
+    KernelProfiler.reset()
     t0 = time.perf_counter()
     outs = model.beam_search(prompts, params) if a.batch else [model.beam_search(p, params) for p in prompts]
     wall = time.perf_counter() - t0
@@ -138,6 +146,7 @@ def _beam_search(a, model, prompts) -> int:
         with open(a.jsonl_output, "w") as f:
             for r in rows:
                 f.write(json.dumps(r) + "\n")
+    _print_profile(a)
     return 0
 
 

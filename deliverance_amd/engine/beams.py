@@ -18,6 +18,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from ..kernels import ops
+from ..profiler import InferenceProfiler
 from .step import BeamStep, StepEntry
 
 
@@ -191,9 +192,11 @@ class BeamSearch:
                     new.append(_Live(i, BeamGroup(self.params, self.ends, n), B, len(self.cache.groups), p))
                 if new:
                     live += new
-                    self._start(new)
+                    with InferenceProfiler.timer("beam_search.prompts"):
+                        self._start(new)
                 else:
-                    self._advance(live)
+                    with InferenceProfiler.timer("beam_search.step"):
+                        self._advance(live)
                 for w in [w for w in live if w.group.done]:
                     for rid in w.rids:
                         if rid in self.mgr:

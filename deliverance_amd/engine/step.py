@@ -170,6 +170,7 @@ class StepRunner:
         from .native_step import NativeStep
         self.joins_shares = NativeStep.takes(model, cache, kernels)
         self.native = NativeStep(model, cache) if native_step and self.joins_shares else None
+        self._attention_shapes = None                # (cache group, heads, key heads, head size) of the layers, for the native plan's models
         # hook(layer, stage, tensor) for named intermediates of every step; steps then run kernel by
         # kernel, never from a recorded graph
         self.debug_hook = None
@@ -368,9 +369,13 @@ class StepRunner:
     def _beams_attend(self, ctx) -> bool:
         """Whether attention of this step reads what beams share once (``ops.attention_beams``): the calls that are issued from C++
         do not know of it."""
+        if ctx.n_beams < 2:
+            return False
         from ..kernels import ops
-        return ctx.n_beams > 1 and any(ops.attention_beams_pays(ctx, ctx.group_of(c.cache), blk.n_heads, blk.n_kv_heads, blk.head_dim, self.cache.page_size)
-                                       for c in self.model.config.schedule for blk in (self.model.blocks[c.layer].mixer,))
+        if self._attention_shapes is None:
+            mixers = [(c, self.model.blocks[c.layer].mixer) for c in self.model.config.schedule]
+            self._attention_shapes = {(ctx.group_of(c.cache), m.n_heads, m.n_kv_heads, m.head_dim) for c, m in mixers}
+        return any(ops.attention_beams_pays(ctx, *shape, self.cache.page_size) for shape in self._attention_shapes)
 
     def _context(self, dev, offs, meta, arena) -> StepContext:
         def view(name):

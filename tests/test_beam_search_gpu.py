@@ -181,3 +181,11 @@ def test_beam_search_from_the_command_line(models, tmp_path):
     assert p.returncode == 0, p.stderr
     row = json.loads(out.read_text())
     assert len(row["hypotheses"]) == 3 and [int(t) for t in p.stdout.strip().split(",")] == row["hypotheses"][0]["token_ids"]
+
+
+def test_profile_of_a_beam_search(models):
+    p = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "deliverance"), "generate", "--model", models["A"].folder, "--prompt-ids", "5,17,3",
+                        "--num-beams", "3", "--max-tokens", "8", "--ignore-eos", "--working-dtype", "F32", "--max-cached-tokens", "512", "--profile-stages"],
+                       capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr
+    assert all(word in p.stderr for word in ("profile summary", "beam_search.prompts", "beam_search.step", "beam_select", "state_reorder"))
