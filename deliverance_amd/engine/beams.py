@@ -25,7 +25,7 @@ from .step import BeamStep, StepEntry
 @dataclass
 class BeamParameters:
     """``num_beams`` continuations of up to ``max_tokens`` tokens (``ntokens`` bounds prompt + generated positions, as in
-    ``GeneratorParameters``); hypotheses are ranked by score / length ** ``length_penalty`` (length: generated tokens).  The search of a
+    ``GeneratorParameters``); hypotheses are ranked by score / length ** ``length_penalty`` (-32 to 32; length: generated tokens).  The search of a
     prompt ends when it has ``num_beams`` finished hypotheses and no live beam's score / length ** ``length_penalty`` is better than
     the worst of them, or, with ``early_stopping``, as soon as it has them."""
     num_beams: int = 4
@@ -44,8 +44,8 @@ class BeamParameters:
             raise ValueError("max_tokens must be positive")
         if self.ntokens is not None and self.ntokens <= 0:
             raise ValueError("ntokens must be positive")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be finite")
+        if not abs(self.length_penalty) <= 32:             # (the power of a length must be a number, and not 0)
+            raise ValueError("length_penalty must be in -32..32")
 
     def candidates(self, n_ends: int) -> int:
         """So many that ``num_beams`` of them go on, whichever end."""

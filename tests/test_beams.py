@@ -238,6 +238,20 @@ def test_operands_on_another_device_are_refused(monkeypatch):
         ops._dev_here(Operand(1), Operand(-1))
 
 
+def test_length_penalties_whose_power_is_no_number_are_refused():
+    from deliverance_amd.engine.beams import BeamGroup, BeamParameters
+    for bad in (32.5, -400.0, 1e6, math.inf):              # (400 tokens: 10^1040, no float; -400: zero, a division by it)
+        with pytest.raises(ValueError, match="length_penalty"):
+            BeamParameters(length_penalty=bad).validate(1)
+    for good in (32.0, -32.0):
+        params = BeamParameters(num_beams=2, length_penalty=good)
+        params.validate(1)
+        group = BeamGroup(params, {7}, 10 ** 6)
+        group.tokens = [[1] * (10 ** 6 - 1)] * 2
+        group.take([(-1e5, 0, 7), (-1.1e5, 1, 7), (-2e5, 0, 3), (-2e5, 1, 3)])
+        assert all(math.isfinite(h.rank) and h.rank < 0 for h in group.finished) and len(group.finished) >= 2
+
+
 def test_entry_points_refuse_sizes_before_they_launch():
     """Sizes outside the kernels' limits end with a message, whatever the pointers (no GPU is touched)."""
     from deliverance_amd.kernels import build, ops
