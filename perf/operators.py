@@ -217,7 +217,8 @@ def run(state):
             return {"scores": scores, "parents": parents, "tokens": tokens}
         if case["op"] == "reorder":
             return ops.state_reorder(state["tensors"], state["slots"], state["parents"], dim=1 if case["stacked"] else 0)
-        splits = ops.beam_splits(case["groups"], case["beams"], case["heads"], case["kv_heads"], case["dim"], state["table"].shape[1], case["page"])
+        splits = ops.beam_splits(case["groups"], case["beams"], case["heads"], case["kv_heads"], case["dim"], state["table"].shape[1], case["page"],
+                                 TYPES[case["dtype"]])
         return ops.attention_beams(state["q"], state["cache"], state["table"], state["lens"], state["shared"], case["beams"], case["heads"],
                                    case["dim"] ** -0.5, None, state["out"], splits, state["scratch"])
     return {"select": _select, "reorder": _reorder, "attention": _attention}[case["op"]](state)
