@@ -5,8 +5,11 @@
 //
 // A logit that is -inf or no number is never chosen and adds nothing to the sum; a score that is -inf or no number marks a
 // place without a beam; where the largest logit is infinite, the entries that reach it share the probability.  Keys are 64-bit: a
-// 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  The terms of the sum are 32-bit exponentials;
-// four that lie side by side are added in 32-bit (two roundings of 2^-24), the rest in 64-bit.
+// 32-bit sum of a score near -100 and a logit makes neighbouring logits equal.  Scores come and go as 32-bit numbers, alone or with what
+// they leave of the 64-bit sum as a second one (together 48 bits): a search that hands one choice's scores to the next as 32-bit numbers
+// alone rounds at the size of the whole sum with every token (1,000 tokens of 3 nats: off by 1e-3, more than many beams are apart).
+// The terms of the sum are 32-bit exponentials; four that lie side by side are added in 32-bit (two roundings of 2^-24), the rest in
+// 64-bit: a logarithm of a sum, and so the distance of keys of two beams, is good to 2^-21.
 //
 // Two kernels.  beam_stats_kernel crosses the logits once: a wavefront takes 512 or 1,024 logits of a row and leaves their maximum
 // and sum, and the largest of each segment of 64 or 256.  beam_choose_kernel, one workgroup a group, works on what is left, by a bound
@@ -193,9 +196,10 @@ __device__ void narrow(Chosen& bound, uint64_t largest, int keep, int most, Coun
 // HELD: segments whose keys a thread keeps (those behind them it works out again)
 template <int SEG, int HELD>
 __global__ void __launch_bounds__(CHOOSE_THREADS)
-beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int K, const float* __restrict__ scores, int n_segs,
-                   int n_parts, const float* __restrict__ seg_max, const float* __restrict__ part_max, const double* __restrict__ part_sum,
-                   float* __restrict__ out_score, int* __restrict__ out_parent, int* __restrict__ out_token, uint32_t magic) {
+beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int K, const float* __restrict__ scores,
+                   const float* __restrict__ scores_low, int n_segs, int n_parts, const float* __restrict__ seg_max, const float* __restrict__ part_max, const double* __restrict__ part_sum,
+                   float* __restrict__ out_score, float* __restrict__ out_low, int* __restrict__ out_parent, int* __restrict__ out_token,
+                   uint32_t magic) {
   constexpr int SEG_LANES = SEG / 4, SIDE = DA_WAVE / SEG_LANES;      // a segment's lanes, 4 entries each; segments of a wavefront side by side
   __shared__ double base[BEAM_MAX], logsum[BEAM_MAX];     // the score (-inf: no beam); the logarithm of the sum
   __shared__ float top[BEAM_MAX];
@@ -217,7 +221,7 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
   for (int b = wave; b < B; b += CHOOSE_WAVES) {
     const float* pm = part_max + (row0 + b) * n_parts;
     const double* ps = part_sum + (row0 + b) * n_parts;
-    const float sc = scores[row0 + b];
+    const double sc = (double)scores[row0 + b] + (scores_low ? (double)scores_low[row0 + b] : 0.0);
     // (a lane past the end takes the last part's maximum again, and no sum)
     const float p0 = pm[min(lane, n_parts - 1)], p1 = pm[min(lane + DA_WAVE, n_parts - 1)];
     const double s0 = ps[min(lane, n_parts - 1)], s1 = ps[min(lane + DA_WAVE, n_parts - 1)];
@@ -230,7 +234,7 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     s = wave_sum_d(m > -INFINITY ? s : 0.0);
     if (lane == 0) {
       top[b] = m;
-      base[b] = (m > -INFINITY && sc == sc) ? (double)sc : -INFINITY;
+      base[b] = (m > -INFINITY && sc == sc) ? sc : -INFINITY;
       logsum[b] = s > 0.0 ? log(s) : 0.0;
     }
   }
@@ -393,13 +397,17 @@ beam_choose_kernel(const float* __restrict__ logits, long ldl, int V, int B, int
     for (int j = t % 4; j < n_entries; j += 4) r += in_front(list[j].key, list[j].place, mine.key, mine.place);
     r = sum_of_lanes(r, 4);
     if (t % 4 == 0 && i < n_entries && r < K) {
-      out_score[(size_t)g * K + r] = (float)unordered64(mine.key);
+      const double sc = unordered64(mine.key);
+      const float near = (float)sc;
+      out_score[(size_t)g * K + r] = near;
+      if (out_low) out_low[(size_t)g * K + r] = fabsf(near) < INFINITY ? (float)(sc - (double)near) : 0.f;
       out_parent[(size_t)g * K + r] = mine.place / V;
       out_token[(size_t)g * K + r] = mine.place % V;
     }
   }
   if (t >= n_entries && t < K) {
     out_score[(size_t)g * K + t] = -INFINITY;
+    if (out_low) out_low[(size_t)g * K + t] = 0.f;
     out_parent[(size_t)g * K + t] = -1;
     out_token[(size_t)g * K + t] = -1;
   }
@@ -428,8 +436,10 @@ extern "C" int da_beam_select_words(int G, int B, int V) {
   return words > 0x7fffffffL ? -1 : (int)words;
 }
 
-extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V, const float* scores, int K, float* out_score,
-                              int* out_parent, int* out_token, float* scratch, long scratch_words, void* stream) {
+// scores_low, out_low: what the scores leave of the 64-bit sums (null: nothing).
+extern "C" int da_beam_select_low(const float* logits, long ldl, int G, int B, int V, const float* scores, const float* scores_low, int K,
+                                  float* out_score, float* out_low, int* out_parent, int* out_token, float* scratch, long scratch_words,
+                                  void* stream) {
   DA_REQUIRE(G >= 0 && B > 0 && B <= BEAM_MAX && V > 0 && ldl >= V && (long)B * V <= 0x7fff0000L,
              "beam_select: bad sizes (groups=%d beams=%d vocabulary=%d row length %ld; at most %d beams)", G, B, V, ldl, BEAM_MAX);
   DA_REQUIRE(K > 0 && K <= BEAM_MAX_KEEP, "beam_select: %d candidates (1 to %d)", K, BEAM_MAX_KEEP);
@@ -455,12 +465,17 @@ extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V
   // i * magic / 2^32 is i / n_segs while i < 2^16 and n_segs < 2^16: the product's error, i * (magic * n_segs - 2^32) / n_segs / 2^32, is below i / 2^32
   const uint32_t magic = (long)B * n_segs < 65536 && n_segs > 1 ? (uint32_t)(((1ull << 32) + n_segs - 1) / n_segs) : 0;
 #define DA_CHOOSE(SEG, HELD) \
-  hipLaunchKernelGGL((beam_choose_kernel<SEG, HELD>), dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, n_segs, n_parts, \
-                     seg_max, part_max, part_sum, out_score, out_parent, out_token, magic)
+  hipLaunchKernelGGL((beam_choose_kernel<SEG, HELD>), dim3(G), dim3(CHOOSE_THREADS), 0, (hipStream_t)stream, logits, ldl, V, B, K, scores, scores_low, n_segs, n_parts, \
+                     seg_max, part_max, part_sum, out_score, out_low, out_parent, out_token, magic)
   if (cut.seg == 64) DA_CHOOSE(64, 2);
   else if (B * n_segs <= 2 * CHOOSE_THREADS) DA_CHOOSE(256, 2);
   else DA_CHOOSE(256, 4);                               // (32 x 8 beams, 131,071: 34.4 us for 37.1)
 #undef DA_CHOOSE
   DA_CHECK_LAUNCH("beam_select (choice)");
   return 0;
+}
+
+extern "C" int da_beam_select(const float* logits, long ldl, int G, int B, int V, const float* scores, int K, float* out_score,
+                              int* out_parent, int* out_token, float* scratch, long scratch_words, void* stream) {
+  return da_beam_select_low(logits, ldl, G, B, V, scores, nullptr, K, out_score, nullptr, out_parent, out_token, scratch, scratch_words, stream);
 }

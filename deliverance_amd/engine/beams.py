@@ -248,16 +248,19 @@ class BeamSearch:
     def _first_choice(self, group: List[_Live], logits: torch.Tensor) -> None:
         """Among one row of logits a prompt.  (The rows go in one by one as groups of one beam.)"""
         n, dev = len(group), logits.device
-        chosen = torch.empty(3, n, self.n_keep, dtype=torch.int32, device=dev)
+        chosen = torch.empty(4, n, self.n_keep, dtype=torch.int32, device=dev)
         ws = torch.empty(ops.beam_select_floats(n, 1, logits.shape[1]), device=dev)
-        ops.beam_select(logits, torch.zeros(n, device=dev), 1, chosen[0].view(torch.float32), chosen[1], chosen[2], ws)
+        ops.beam_select(logits, torch.zeros(n, device=dev), 1, chosen[0].view(torch.float32), chosen[1], chosen[2], ws,
+                        out_scores_low=chosen[3].view(torch.float32))
         for w, c in zip(group, self._candidates(chosen)):
             w.group.take(c)
 
     @staticmethod
     def _candidates(chosen: torch.Tensor) -> List[List[Tuple[float, int, int]]]:
-        scores, parents, tokens = chosen.cpu()
-        return [list(zip(s, p, t)) for s, p, t in zip(scores.contiguous().view(torch.float32).tolist(), parents.tolist(), tokens.tolist())]
+        """(score, parent, token) of every place; a score is the sum of its two 32-bit parts."""
+        scores, parents, tokens, low = chosen.cpu()
+        scores = scores.contiguous().view(torch.float32).double() + low.contiguous().view(torch.float32).double()
+        return [list(zip(s, p, t)) for s, p, t in zip(scores.tolist(), parents.tolist(), tokens.tolist())]
 
     def _advance(self, live: List[_Live]) -> None:
         """One token of every beam of every prompt, and the next choice."""

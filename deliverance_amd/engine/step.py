@@ -221,8 +221,8 @@ class StepRunner:
         sequences only, the step and its sampling are replayed from a recorded HIP graph and the
         sampled tokens are left in ``ctx.sampled`` (the first rows of ``self.sampled``).  With ``beams`` (in place of
         ``sample_records``) the step's entries are beams, one token each whose logits are wanted, and the choice of the next ones
-        (``ops.beam_select``) is left in ``ctx.chosen``, int32 [3, requests, n_keep] on the device: the bits of the 32-bit scores, parents
-        and tokens."""
+        (``ops.beam_select``) is left in ``ctx.chosen``, int32 [4, requests, n_keep] on the device: the bits of the 32-bit scores, parents,
+        tokens, and the bits of what the scores leave of the 64-bit sums."""
         mgr = self.cache.manager
         cfg = self.model.config
         if not entries:
@@ -322,6 +322,15 @@ class StepRunner:
             words += list(per_request) + [0] * (n_requests - len(per_request))
         return words
 
+    @staticmethod
+    def _beam_low_words(beams: BeamStep, n_requests: int) -> List[int]:
+        """What the 32-bit scores of ``_beam_words`` leave of the beams' scores, as the bits of 32-bit floats."""
+        scores = np.asarray(beams.scores, dtype=np.float64)
+        near = scores.astype(np.float32)
+        low = np.zeros(n_requests * beams.n_beams, dtype=np.float32)
+        np.subtract(scores, near, out=low[:len(scores)], where=np.isfinite(near), casting="same_kind")
+        return low.view(np.int32).tolist()
+
     def _take_beams(self, ctx, beams: BeamStep) -> None:
         """Where the step's arrays of beam search lie in ``ctx.extra``."""
         n, G = ctx.n_seqs, len(self.cache.groups)
@@ -330,18 +339,23 @@ class StepRunner:
         ctx.beam_scores = ctx.extra[:n].view(torch.float32)
         ctx.beam_shared_host = beams.shared
         ctx.beam_shared = [ctx.extra[n + g * per:n + (g + 1) * per] for g in range(G)]
+        ctx.beam_scores_low = ctx.extra[n + G * per:2 * n + G * per].view(torch.float32)
 
     def _choose(self, ctx, beams: BeamStep, logits: torch.Tensor):
         from ..kernels import ops
         per = ctx.n_seqs // beams.n_beams
-        chosen = ctx.flat("beam_chosen", 3 * per * beams.n_keep, torch.int32).view(3, per, beams.n_keep)
+        chosen = ctx.flat("beam_chosen", 4 * per * beams.n_keep, torch.int32).view(4, per, beams.n_keep)
         ws = ctx.flat("beam_select", ops.beam_select_floats(logits.shape[0], beams.n_beams, logits.shape[1]), torch.float32)
-        ops.beam_select(logits, ctx.beam_scores, beams.n_beams, chosen[0].view(torch.float32), chosen[1], chosen[2], ws)
+        ops.beam_select(logits, ctx.beam_scores, beams.n_beams, chosen[0].view(torch.float32), chosen[1], chosen[2], ws,
+                        ctx.beam_scores_low, chosen[3].view(torch.float32))
         return chosen
 
     def _run_eager(self, entries, order, starts, sample_records, beams=None):
         from ..kernels import ops
-        extra = sample_records if beams is None else self._beam_words(beams, len(entries) // beams.n_beams)
+        extra = sample_records
+        if beams is not None:
+            n = len(entries) // beams.n_beams
+            extra = self._beam_words(beams, n) + self._beam_low_words(beams, n)
         offs, meta, n_words = self._layout(entries, order, pad_to=None, max_blocks=None, extra=extra)
         self._fill(self._staging_for(n_words), offs, meta, entries, order, starts, extra)
         dev = self._upload(n_words)
@@ -413,7 +427,9 @@ class StepRunner:
         while bucket < S:
             bucket *= 2
         order = list(range(S))
-        extra, a_pad = (sample_records, RECORD_WORDS) if beams is None else (self._beam_words(beams, bucket // unit), 0)
+        extra, a_pad = sample_records, RECORD_WORDS
+        if beams is not None:
+            extra, a_pad = self._beam_words(beams, bucket // unit) + self._beam_low_words(beams, bucket // unit), 0
         offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap, extra=extra, extra_a_pad=a_pad)
         key = bucket if beams is None else (bucket, beams.n_beams, beams.n_keep)
         st = self._graphs.get(key)

@@ -186,6 +186,7 @@ _ARGTYPES = {
                          _VP, ctypes.c_long, _VP],
     "da_beam_select_words": [_I, _I, _I],
     "da_beam_select": [_VP, ctypes.c_long, _I, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, ctypes.c_long, _VP],
+    "da_beam_select_low": [_VP, ctypes.c_long, _I, _I, _I, _VP, _VP, _I, _VP, _VP, _VP, _VP, _VP, ctypes.c_long, _VP],
     "da_state_reorder": [_VP, _I, _I, _VP, _VP, _I, _I, _VP],
     "da_attn_beams_takes": [_I, _I],
     "da_attn_beams_splits": [_I, _I, _I, _I, _I, _I, _I, _I],
@@ -859,32 +860,39 @@ def beam_select_floats(n_rows: int, n_beams: int, vocab: int) -> int:
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_parents: torch.Tensor,
-                out_tokens: torch.Tensor, workspace: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                out_tokens: torch.Tensor, workspace: torch.Tensor, scores_low: Optional[torch.Tensor] = None,
+                out_scores_low: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The choice of beam search: rows g * n_beams + b of ``logits`` (float32) are the beams of group g, ``scores`` (float32, one a
     row) their summed log-probabilities.  Of every group the K = out_scores.shape[1] pairs (beam, token) with the largest
     score + log-probability go to ``out_scores`` (float32), ``out_parents`` and ``out_tokens`` (int32), all [G, K], in descending order,
     the lowest beam and then the lowest token first among equals.  A score of -inf marks a place without a beam, a logit of -inf a
     token that must not be chosen (no number counts as -inf in both); candidates that do not exist are (-inf, -1, -1).
-    ``workspace``: float32, ``beam_select_floats`` elements."""
-    _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace)
+    ``workspace``: float32, ``beam_select_floats`` elements.  Sums are 64-bit inside.  Where choices follow one another, what a
+    float32 score leaves of its sum goes to ``out_scores_low`` (like ``out_scores``; 0 for an infinite score) and comes back as ``scores_low``
+    (like ``scores``): score + low carries 48 bits, where a score alone is rounded at the size of the whole sum with every token."""
+    _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace, scores_low, out_scores_low)
     _rows_2d(logits, "logits")
     R, V = logits.shape
     if not 1 <= n_beams <= MAX_BEAMS or R % n_beams:
         raise KernelError(f"beam_select: {R} rows in groups of {n_beams} (1 to {MAX_BEAMS})")
     if logits.dtype != torch.float32 or scores.dtype != torch.float32 or scores.numel() != R or not scores.is_contiguous():
         raise KernelError("beam_select: logits and scores must be float32, one score a row")
+    if scores_low is not None and (scores_low.dtype != torch.float32 or scores_low.numel() != R or not scores_low.is_contiguous()):
+        raise KernelError("beam_select: scores_low must be float32, one a row")
     shape = (R // n_beams, out_scores.shape[-1] if out_scores.dim() else 0)
     if not 1 <= shape[1] <= MAX_CANDIDATES:
         raise KernelError(f"beam_select: {shape[1]} candidates (1 to {MAX_CANDIDATES})")
-    for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32)):
+    low = out_scores if out_scores_low is None else out_scores_low
+    for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32), (low, torch.float32)):
         if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
             raise KernelError(f"beam_select: outputs must be contiguous {list(shape)}, float32 scores and int32 parents and tokens")
     if workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise KernelError("beam_select: the workspace must be contiguous float32")
     G, K = shape
     with _timed("beam_select", 4 * R * V, 4 * R * V, "fp32"):
-        _check(_lib().da_beam_select(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), K, _ptr(out_scores), _ptr(out_parents),
-                                     _ptr(out_tokens), _ptr(workspace), workspace.numel(), _stream()))
+        _check(_lib().da_beam_select_low(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), _ptr(scores_low), K, _ptr(out_scores),
+                                         _ptr(out_scores_low), _ptr(out_parents), _ptr(out_tokens), _ptr(workspace), workspace.numel(),
+                                         _stream()))
     return out_scores, out_parents, out_tokens
 
 

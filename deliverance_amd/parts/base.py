@@ -119,12 +119,14 @@ class StepContext:
         self.block_tables: List[torch.Tensor] = []     # per group int32 [S, max_blocks]
         self.slot_maps: List[torch.Tensor] = []        # per group int32 [N]
         # Beam search: the step's sequences are groups of ``n_beams`` whose tables begin with the same pages (0: they are not);
-        # per cache group int32 [S / n_beams], how many positions those pages hold; the beams' summed log-probabilities, float32 [S]
+        # per cache group int32 [S / n_beams], how many positions those pages hold; the beams' summed log-probabilities, float32 [S], and what
+        # these leave of the 64-bit sums
         self.n_beams = 0
         self.beam_shared: List[torch.Tensor] = []
         self.beam_shared_host: List[List[int]] = []
         self.beam_scores: torch.Tensor = None
-        self.chosen: torch.Tensor = None               # int32 [3, S / n_beams, candidates], what the step's choice left (engine/step.py)
+        self.beam_scores_low: torch.Tensor = None
+        self.chosen: torch.Tensor = None               # int32 [4, S / n_beams, candidates], what the step's choice left (engine/step.py)
         self.cache = None                              # engine.DeviceCache
         self._arena = None
         # False while a part runs that was given a buffer of its own to fill (a norm follows it): a part

@@ -301,3 +301,21 @@ def test_entry_points_refuse_sizes_before_they_launch():
     refused(attend(splits=2), "workspace")
     refused(attend(splits=2, ws=64, floats=2 * 2 * 2 * 34 - 1), "workspace")
     assert attend(G=0) == 0
+
+
+def test_a_beams_score_goes_to_the_device_in_two_parts():
+    import torch
+    from deliverance_amd.engine.beams import BeamSearch
+    from deliverance_amd.engine.step import BeamStep, StepRunner
+    scores = [-12345.678901234, -math.inf, -1.0 / 3.0, 0.0]
+    step = BeamStep(2, 4, scores, [[32, 16]])
+    high = np.array(StepRunner._beam_words(step, 3)[:6], dtype=np.int32).view(np.float32).astype(np.float64)
+    low = np.array(StepRunner._beam_low_words(step, 3), dtype=np.int32).view(np.float32).astype(np.float64)
+    assert low.shape == (6,) and low[[1, 3, 4, 5]].tolist() == [0.0] * 4 and high[1] == high[4] == -math.inf
+    assert all(abs(high[i] + low[i] - scores[i]) <= 2.0 ** -48 * abs(scores[i]) for i in (0, 2, 3))
+    # and back: int32 [4, requests, candidates], score, parent, token, what the score leaves
+    chosen = torch.tensor([np.float32(high[[0, 2, 1]]).view(np.int32).tolist(), [1, 0, -1], [7, 3, -1],
+                           np.float32(low[[0, 2, 1]]).view(np.int32).tolist()], dtype=torch.int32).view(4, 1, 3)
+    (a, b, none), = BeamSearch._candidates(chosen)
+    assert a[1:] == (1, 7) and b[1:] == (0, 3) and none == (-math.inf, -1, -1)
+    assert abs(a[0] - scores[0]) <= 2.0 ** -48 * abs(scores[0]) and abs(b[0] - scores[2]) <= 2.0 ** -48
