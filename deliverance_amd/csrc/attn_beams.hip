@@ -14,8 +14,9 @@
 //   values : O^T[d, row] += V^T[d, key] P^T[key, row].  Values lie dimension by dimension, so the left operand is read as it lies;
 //            which key stands in which row of the first product is chosen so that a lane's weights are the ones that the second
 //            takes from it: nothing is exchanged.
-// bfloat16: a 32-bit weight goes in as two bfloat16 parts (16 bits; with one part the result is off by 1.91e-3 in place of 1.66e-3, its own
-// rounding, and 8 x 8 beams over 1,003 positions take 17.1 us in place of 17.5).  32-bit: 16x16x4 products, nothing is rounded.
+// bfloat16: a 32-bit weight goes in as three bfloat16 parts, which lose nothing (3 x 8 bits), as in the decode kernel that takes the step
+// otherwise: with two, small differences of weights are off by more than the result's rounding, for 1 % (8 x 8 beams over 1,003 positions 17.4 us
+// in place of 17.7, 1 x 4 over 531 7.7 in place of 7.8, 4 x 4 over 32,701 the same).  32-bit: 16x16x4 products, nothing is rounded.
 // Bound by memory where contexts are long (4 x 4 beams, 32 / 8 heads of 128, 32,701 positions: 101 us, 5.4 TB/s), else by three round trips, lengths,
 // pages, keys and values, of which the second travels beside the chunk before (4 x 4 beams 124 -> 114 us; 8 x 8 of 25 heads over 1,003 positions 21.4 -> 17.4
 // with 8 wavefronts).  1 x 4 beams of 12 heads over 531 positions: 7.8 us.
@@ -262,19 +263,23 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
             add += e[j][i];
           }
         l[y] = l[y] * alpha + add;
-        uint4 hi[VP], lw[VP];                           // bfloat16: the weights' two parts
+        uint4 part[3][VP];                              // bfloat16: the weights, 3 x 8 bits
         if (!F32) {
 #pragma unroll
           for (int j = 0; j < VP; ++j) {
-            uint32_t h4[4], l4[4];
+            uint32_t p4[3][4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const float x0 = e[2 * j + w / 2][2 * (w % 2)], x1 = e[2 * j + w / 2][2 * (w % 2) + 1];
-              h4[w] = pack2_bf16(x0, x1);
-              l4[w] = pack2_bf16(x0 - __uint_as_float(h4[w] << 16), x1 - __uint_as_float(h4[w] & 0xffff0000u));
+              float x0 = e[2 * j + w / 2][2 * (w % 2)], x1 = e[2 * j + w / 2][2 * (w % 2) + 1];
+#pragma unroll
+              for (int p = 0; p < 3; ++p) {
+                p4[p][w] = pack2_bf16(x0, x1);
+                x0 -= __uint_as_float(p4[p][w] << 16);
+                x1 -= __uint_as_float(p4[p][w] & 0xffff0000u);
+              }
             }
-            hi[j] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-            lw[j] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) part[p][j] = make_uint4(p4[p][0], p4[p][1], p4[p][2], p4[p][3]);
           }
         }
 #pragma unroll
@@ -301,8 +306,9 @@ attn_beams_kernel(const T* __restrict__ q, int q_ld, const T* __restrict__ cache
               for (int x = 0; x < 4; ++x) o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v4[x]), e[j][x], o, 0, 0, 0);
             } else {
               const uint4 v = make_uint4(v4[0], v4[1], v4[2], v4[3]);
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, hi[j]), o, 0, 0, 0);
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, lw[j]), o, 0, 0, 0);
+#pragma unroll
+              for (int p = 0; p < 3; ++p)
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, part[p][j]), o, 0, 0, 0);
             }
           }
           // (a column that takes no part keeps its sums: zero times another beam's infinite value is no number)
