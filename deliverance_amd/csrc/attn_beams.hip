@@ -443,6 +443,60 @@ static int beam_waves(long groups, int splits, int max_blocks, int page) {
   return groups * splits > 256 || (long)max_blocks * page / CHUNK >= 48L * splits ? 4 : 8;
 }
 
+// Whether a step of beams is ahead here or in the kernels that take a sequence by itself (bfloat16 attn_decode.hip, 32-bit attn_f32.hip): both sides' times,
+// us, from the step's shape and what its sequences see.  A start; what joining shares adds; then the larger of the workgroups' chains (rounds of 64 or 32
+// keys a wavefront, and one for the way in and out) where compute units take several in turn, and the bytes that are asked for (here those of shared keys
+// once a workgroup; much of it comes from caches).  The numbers are fitted to 20,584 measured pairs: 2 to 32 beams, 1 to 16 groups, 2 to 32 heads of 16 to 256, 1 to 8 of
+// them a key head, 11 to 32,000 positions in tables up to 32,768 wide, windows from 64.  Of those the choice is the faster kernel or within 5 % of it in 92 of 100, 1.3 % behind it on
+// average, 1.84 times at the worst (one by the table's width alone: 60 of 100, 18 %, 14.5 times).  us, the others / here: bfloat16, 2 x 3 beams of 4 heads of 16 in a
+// table of 2,048 positions: 23 positions 6.5 / 7.5, 547 7.7 / 7.6; 4 x 32 of 25 heads of 64, 393 37.8 / 23.3; 1 x 3 of 32 / 8 heads of 128, 102 5.0 / 9.4; 8 x 5 of 8 / 1
+// heads of 64, 23 in 4,096 4.7 / 9.0; 1 x 4 of 12 heads of 64, 531 5.4 / 7.8, 4,000 12.1 / 9.3; 32-bit: 1 x 4 of 2 heads of 48, 33 5.1 / 10.4; 1 x 8 of 8 heads of 128, a window of 64 7.9 / 14.8;
+// 1 x 3 of 12 heads of 64, 3,989 68.9 / 17.7.
+struct StepTime {
+  float units, units_wide;       // of a compute unit, that a workgroup takes: head sizes up to 64, above
+  float start, start_d;          // _d: for each 64 of the head size
+  float join, join_share;
+  float round, round_d;
+  float megabyte;
+};
+static float step_us(const StepTime& t, int D, int d, int shares, float workgroups, float rounds, float megabytes) {
+  const float in_turn = workgroups / 256 * (d <= 64 ? t.units : t.units_wide), d64 = d / 64.f;
+  const float chain = (in_turn > 1 ? in_turn : 1) * (rounds + 1) * (t.round + t.round_d * d64), bytes = megabytes * t.megabyte;
+  return t.start + t.start_d * d64 + (shares > 1 ? t.join + t.join_share * shares * da_ceil_div(D, 64) : 0) + (chain > bytes ? chain : bytes);
+}
+
+// By how many nanoseconds a step is ahead here (negative: behind; where the two are within 6 % it stays here, where nothing is read twice).  visible:
+// positions that a sequence sees, shared: those of them that its group shares, both on average; decode_splits: shares of the other kernel (bfloat16).
+extern "C" int da_attn_beams_ahead_ns(int G, int B, int Hq, int Hkv, int D, int dtype, int max_blocks, int page, int splits, int decode_splits,
+                                      int visible, int shared) {
+  if (G <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_blocks <= 0 || splits <= 0 || decode_splits <= 0 || visible <= 0 || !da_attn_beams_takes(D, page)) return -1;
+  static const StepTime decode_bf16 = {0.69f, 1.43f, 1.97f, 0.403f, 2.36f, 0.189f, 1.71f, 0.305f, 0.112f};
+  static const StepTime decode_f32 = {0.72f, 0.956f, 1.36f, 0.f, 0.f, 0.f, 2.06f, 1.96f, 0.146f};
+  static const StepTime beams_bf16 = {0.909f, 0.817f, 2.08f, 0.044f, 2.56f, 0.0617f, 1.52f, 1.05f, 0.204f};
+  static const StepTime beams_f32 = {0.891f, 0.686f, 0.f, 0.f, 3.52f, 0.0611f, 2.31f, 3.38f, 0.221f};
+  const bool f32 = dtype == DA_F32;
+  const float S = (float)G * B, v = visible, s = shared < visible ? (shared > 0 ? shared : 0) : visible, key_mb = 2.f * D * (f32 ? 4 : 2) * 1e-6f;
+  // the others: a workgroup a (sequence, head, share); shares are by the table's width, so that a short context lies in the first
+  float span = 1e9f, a_wave = 32.f * 8;
+  if (!f32) {
+    span = (float)((((long)max_blocks * page + decode_splits - 1) / decode_splits + CHUNK - 1) / CHUNK * CHUNK);
+    a_wave = (float)CHUNK * (S * Hq * decode_splits <= 256 && D <= 64 ? 16 : 8);
+  }
+  const float with_keys = v / span < 1 ? 1 : (v / span > decode_splits ? decode_splits : v / span);
+  const float others = step_us(f32 ? decode_f32 : decode_bf16, D, D, f32 ? 1 : decode_splits, S * Hq * (f32 ? 1 : with_keys), (v < span ? v : span) / a_wave, S * Hq * v * key_mb);
+  // here: the shared chunks and those of the beams whose rows a workgroup has, whole ones
+  const int rows = beam_rows(G, B, Hq, Hkv, D), ratio = Hq / Hkv;
+  const float groups = (float)beam_groups(G, B, Hq, Hkv, rows), beams = rows < B * ratio ? (float)rows / ratio : (float)B;
+  const float chunks = s / CHUNK + beams * ((v - s) / CHUNK + 0.75f);
+  const float once = G * (s + B * (v - s)) * Hkv, asked = 0.8f * groups * (s + beams * (v - s));
+  const int waves = D > 128 ? 4 : (rows > TILE ? 8 : beam_waves((long)groups, splits, max_blocks, page));
+  const float joined_mb = splits > 1 ? S * Hq * splits * D * 8e-6f : 0.f;
+  const float here = step_us(f32 ? beams_f32 : beams_bf16, D, D <= 32 ? 32 : (D <= 64 ? 64 : (D <= 128 ? 128 : 256)), splits, groups * splits,
+                             chunks / splits / waves, (once > asked ? once : asked) * key_mb) + joined_mb * (f32 ? 0.482f : 0.381f);
+  const float ns = (1.06f * others - here) * 1000;
+  return ns > 1e9f ? 1000000000 : (ns < -1e9f ? -1000000000 : (int)ns);
+}
+
 template <typename T, int DK, int STEP>
 static void beams_launch(hipStream_t s, const void* q, int q_ld, const void* cache, const int* block_table, int max_blocks, const int* seq_lens,
                          const int* shared, int G, int B, int Hq, int Hkv, int D, int page, float scale, int window, void* out, int out_ld,

@@ -170,7 +170,8 @@ class StepRunner:
         from .native_step import NativeStep
         self.joins_shares = NativeStep.takes(model, cache, kernels)
         self.native = NativeStep(model, cache) if native_step and self.joins_shares else None
-        self._attention_shapes = None                # (cache group, heads, key heads, head size) of the layers, for the native plan's models
+        # (cache group, heads, key heads, head size, window) of the layers whose beams' shared pages can be read once
+        self._beam_layers: Optional[List[tuple]] = None
         # hook(layer, stage, tensor) for named intermediates of every step; steps then run kernel by
         # kernel, never from a recorded graph
         self.debug_hook = None
@@ -362,6 +363,7 @@ class StepRunner:
         ctx = self._context(dev, offs, meta, self.arena)
         if beams is not None:
             self._take_beams(ctx, beams)
+            ctx.beams_attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries], meta["S"], meta["max_blocks"], recorded=False)
         ctx.debug_hook = self.debug_hook
         self.last_ctx = ctx
         R = meta["R"]
@@ -376,20 +378,37 @@ class StepRunner:
         """The model's forward pass of this step: from C++ in one call, or part by part (always with the
         debug hook or the kernel profiler, which look between the kernels)."""
         from ..profiler import KernelProfiler
-        if self.native is not None and ctx.debug_hook is None and not KernelProfiler.enabled and not self._beams_attend(ctx):
+        if self.native is not None and ctx.debug_hook is None and not KernelProfiler.enabled and not ctx.beams_attend:
             return self.native.forward(ctx, want_rows, n_want)
         return self.model.forward(ctx, want_rows, n_want)
 
-    def _beams_attend(self, ctx) -> bool:
-        """Whether attention of this step reads what beams share once (``ops.attention_beams``): the calls that are issued from C++
-        do not know of it."""
-        if ctx.n_beams < 2:
-            return False
+    # us that a layer of a step that is not recorded takes the host when it is issued part by part in place of one call into the library
+    # (12 layers, a step of 4 or 64 rows: 0.45 and 1.00 ms, 1.23 and 1.76)
+    PART_BY_PART_US = 46.0
+
+    def _beams_attend(self, beams: BeamStep, lens: Sequence[int], n_seqs: int, max_blocks: int, recorded: bool) -> frozenset:
+        """The layers (``StepContext.beams_attend``) of a step of ``n_seqs`` sequences in tables of ``max_blocks`` pages whose attention reads
+        what beams share once, by what the entries (of ``lens`` positions) see and share.  (The calls that are issued from C++ do not
+        know of it: a step that is not recorded leaves them only for more than that costs the host.)"""
         from ..kernels import ops
-        if self._attention_shapes is None:
-            mixers = [(c, self.model.blocks[c.layer].mixer) for c in self.model.config.schedule]
-            self._attention_shapes = {(ctx.group_of(c.cache), m.n_heads, m.n_kv_heads, m.head_dim) for c, m in mixers}
-        return any(ops.attention_beams_pays(ctx, *shape, self.cache.page_size) for shape in self._attention_shapes)
+        from ..profiler import KernelProfiler
+        if beams.n_beams < 2:
+            return frozenset()
+        if self._beam_layers is None:
+            found = [(self.cache.group_of_slot[c.cache + k], *rest) for c in self.model.config.schedule
+                     for k, *rest in self.model.blocks[c.layer].mixer.paged_attention()]
+            self._beam_layers = sorted(set(found))
+        native = self.native is not None and not recorded and self.debug_hook is None and not KernelProfiler.enabled
+        lens = list(lens)[::beams.n_beams]                   # (a request's beams have one length)
+        attend = set()
+        for group, n_heads, n_kv_heads, head_dim, window in self._beam_layers:
+            gone = [max(0, n - window) if window else 0 for n in lens]
+            visible = sum(n - g for n, g in zip(lens, gone)) // len(lens)
+            shared = sum(max(0, s - g) for s, g in zip(beams.shared[group], gone)) // len(lens)
+            if ops.attention_beams_pays(n_seqs // beams.n_beams, beams.n_beams, n_heads, n_kv_heads, head_dim, self.cache.page_size, max_blocks,
+                                        self.model.dtype, visible, shared, host_us=self.PART_BY_PART_US if native else 0.0):
+                attend.add((group, n_heads, n_kv_heads, head_dim, window))
+        return frozenset(attend)
 
     def _context(self, dev, offs, meta, arena) -> StepContext:
         def view(name):
@@ -431,7 +450,10 @@ class StepRunner:
         if beams is not None:
             extra, a_pad = self._beam_words(beams, bucket // unit) + self._beam_low_words(beams, bucket // unit), 0
         offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap, extra=extra, extra_a_pad=a_pad)
-        key = bucket if beams is None else (bucket, beams.n_beams, beams.n_keep)
+        key, attend = bucket, None
+        if beams is not None:                              # (a step's kernels are recorded: which attention they hold is part of its name)
+            attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries], bucket, self.max_blocks_cap, recorded=True)
+            key = (bucket, beams.n_beams, beams.n_keep, attend)
         st = self._graphs.get(key)
         if st is None:
             host = torch.empty(n_words, dtype=torch.int32, pin_memory=True)
@@ -450,6 +472,7 @@ class StepRunner:
         self.last_ctx = ctx
         if beams is not None:
             self._take_beams(ctx, beams)
+            ctx.beams_attend = attend
 
         sampled = self.sampled[:bucket]
 

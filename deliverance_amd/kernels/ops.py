@@ -190,6 +190,7 @@ _ARGTYPES = {
     "da_state_reorder": [_VP, _I, _I, _VP, _VP, _I, _I, _VP],
     "da_attn_beams_takes": [_I, _I],
     "da_attn_beams_splits": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "da_attn_beams_ahead_ns": [_I] * 12,
     "da_attn_beams": [_VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP, _I, _I, _VP, ctypes.c_long, _VP],
 }
 _LIB = None
@@ -1430,20 +1431,21 @@ def attention_both(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torch
     return out
 
 
-def attention_beams_pays(ctx, group: int, n_heads: int, n_kv_heads: int, head_dim: int, page: int) -> bool:
-    """Whether a step's attention goes to ``attention_beams``: a step of beams, sizes that it takes, the tuned kernels, and, by the step's
-    shape only (a recorded step keeps it), keys enough that reading them once pays for a start that takes longer than the decode
-    kernels'.  us, decode / beams: bfloat16, heads of 64: 8 beams of 12 heads, 1,000 positions 6.4 / 8.0; 8 x 4 of 12 heads, 1,000 (again: 74 MB)
-    11.7 / 11.4; 8 x 2 of 25 heads, 531 (27 MB, one share) 11.3 / 9.5; 8 x 8 of 25 heads, 1,000 (359 MB) 53.8 / 16.7; 2 beams of 12 heads, 4,000
-    12.0 / 9.2; 32-bit: 2 beams of 12 heads, 200 8.0 / 10.2, 531 13.3 / 10.4."""
-    B = getattr(ctx, "n_beams", 0)
-    if _MODE != "tuned" or B < 2 or ctx.n_decode != ctx.n_seqs or not attention_beams_takes(head_dim, page):
+def attention_beams_pays(n_groups: int, n_beams: int, n_heads: int, n_kv_heads: int, head_dim: int, page: int, max_blocks: int,
+                         dtype: torch.dtype, visible: int, shared: int, host_us: float = 0.0) -> bool:
+    """Whether attention of a step of ``n_groups`` x ``n_beams`` sequences, one token each, goes to ``attention_beams``: with the tuned kernels, sizes that
+    it takes, and where its time is below the other kernel's, by the library's estimate (da_attn_beams_ahead_ns in csrc/attn_beams.hip, with both sides
+    measured) from the shape and from the positions that a sequence sees (``visible``) and that its group shares among them (``shared``), on average.
+    Where the other kernel would be the plain one (32-bit head sizes above 128), always.  ``host_us``: what going there costs the host beside."""
+    if _MODE != "tuned" or n_beams < 2 or not attention_beams_takes(head_dim, page):
         return False
-    S, blocks = ctx.n_seqs, ctx.block_tables[group].shape[1]
-    if blocks * page >= 2048 or ctx.dtype == torch.float32:
-        return blocks * page >= 512
-    again = (S * n_heads - S // B * n_kv_heads) * blocks * page * 4 * head_dim      # bytes that the decode kernel would read more than once
-    return again >= (24e6 if beam_splits(S // B, B, n_heads, n_kv_heads, head_dim, blocks, page) == 1 else 100e6)
+    f32 = dtype == torch.float32
+    if f32 and not attention_f32_takes(head_dim, page):
+        return True
+    splits = beam_splits(n_groups, n_beams, n_heads, n_kv_heads, head_dim, max_blocks, page, dtype)
+    others = 1 if f32 else decode_splits(n_groups * n_beams, n_heads, max_blocks, page)
+    return int(_lib().da_attn_beams_ahead_ns(n_groups, n_beams, n_heads, n_kv_heads, head_dim, F32 if f32 else BF16, max_blocks, page, splits, others,
+                                             int(visible), int(shared))) > host_us * 1e3
 
 
 def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, n_heads: int,
@@ -1474,8 +1476,8 @@ def paged_attention(ctx, q: torch.Tensor, cache_slot: torch.Tensor, group: int, 
             pairs += sum(min(n - t + i + 1, window or n) for i in range(t)) if t > 1 else min(n, window or n)
         return keys * 2 * Hkv * D * el + 2 * rows * n_heads * D * el, 4 * pairs * n_heads * D
 
-    if (getattr(ctx, "n_beams", 0) > 1 and attention_beams_pays(ctx, group, n_heads, Hkv, D, page) and q.dtype == ctx.dtype and q.stride(0) * el % 16 == 0
-            and q.data_ptr() % 16 == 0 and cache_slot.data_ptr() % 16 == 0):
+    if (getattr(ctx, "beams_attend", None) and (group, n_heads, Hkv, D, int(window or 0)) in ctx.beams_attend and q.dtype == ctx.dtype
+            and q.stride(0) * el % 16 == 0 and q.data_ptr() % 16 == 0 and cache_slot.data_ptr() % 16 == 0):
         n_splits = beam_splits(nd // ctx.n_beams, ctx.n_beams, n_heads, Hkv, D, bt.shape[1], page, q.dtype)
         ws = ctx.flat("beam_partial", beam_workspace_floats(nd, n_heads, D, n_splits), torch.float32) if n_splits > 1 else None
         nbytes, flops = cost(0, nd)                       # (what a group shares is read once)

@@ -154,6 +154,9 @@ class CausalSelfAttention(Mixer):
                       None if self.v_head_dim == self.head_dim else self.v_head_dim, keep_first=self.keep_first,
                       chunk=self.chunk)
 
+    def paged_attention(self):
+        return () if self.extras else ((0, self.n_heads, self.n_kv_heads, self.head_dim, int(self.window or 0)),)
+
     def kernel_units(self, dtype):
         out = ("attn_prepare",) if self._prepared() else (() if self.position is None else ("attn_latent",))
         if self.v_head_dim != self.head_dim and not self._prepared():

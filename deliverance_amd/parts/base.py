@@ -126,6 +126,8 @@ class StepContext:
         self.beam_shared_host: List[List[int]] = []
         self.beam_scores: torch.Tensor = None
         self.beam_scores_low: torch.Tensor = None
+        # the layers whose attention reads what beams share once (``ops.attention_beams``): (cache group, heads, key heads, head size, window)
+        self.beams_attend: frozenset = frozenset()
         self.chosen: torch.Tensor = None               # int32 [4, S / n_beams, candidates], what the step's choice left (engine/step.py)
         self.cache = None                              # engine.DeviceCache
         self._arena = None
@@ -243,6 +245,11 @@ class Mixer:
 
     def cache_need(self):
         return None
+
+    def paged_attention(self) -> Tuple[tuple, ...]:
+        """(k, query heads, key heads, head size, window or 0) of what the mixer attends by ``ops.paged_attention``, over cache slot
+        ``call.cache + k``: the layers whose beams' shared pages can be read once."""
+        return ()
 
     def forward(self, ctx: StepContext, h: torch.Tensor, x: torch.Tensor, call) -> None:
         raise NotImplementedError

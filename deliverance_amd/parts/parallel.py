@@ -38,6 +38,9 @@ class ParallelMixer(Mixer):
     def cache_need(self):
         return tuple(b.cache_need() for b in self.branches)
 
+    def paged_attention(self):
+        return tuple((k, *rest) for k, b in enumerate(self.branches) for _, *rest in b.paged_attention())
+
     def forward(self, ctx: StepContext, h: torch.Tensor, x: torch.Tensor, call) -> None:
         accumulate = ctx.part_accumulate
         for k, (branch, scale) in enumerate(zip(self.branches, self.scales)):

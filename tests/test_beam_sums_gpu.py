@@ -86,3 +86,27 @@ def test_a_long_search_returns_the_sum_of_its_tokens(graphs, tmp_path):
         z -= z.max(1, keepdims=True)
         want = float((z[np.arange(1500), h.tokens] - np.log(np.exp(z).sum(1))).sum())
         assert abs(h.score - want) <= 1500 * 5e-7
+
+
+@pytest.mark.needs_device
+def test_a_search_takes_the_kernel_that_its_positions_pay_for(tmp_path, monkeypatch):
+    """A model of 2,048 positions: short contexts stay with the decode kernel however wide the tables are, and a search that grows goes over to
+    the kernel that reads shared pages once; a step of either kind is recorded for itself."""
+    import numpy as np
+    import helpers
+    import plain_gpt2 as P
+    from deliverance_amd import AutoModelForCausalLM, BeamParameters
+    m = helpers.make_model(tmp_path, dict(helpers.CONFIG_A, n_positions=2048), seed=5)
+    calls, kernel = [], ops.attention_beams
+    monkeypatch.setattr(ops, "attention_beams", lambda *a, **k: (calls.append(1), kernel(*a, **k))[1])
+    eng = AutoModelForCausalLM.from_pretrained(str(m.folder), dtype="float32", max_cached_tokens=8192, max_num_seqs=4)
+    eng.beam_search(m.prompt(20), BeamParameters(num_beams=3, max_tokens=10, ignore_eos=True))
+    assert not calls
+    prompt = m.prompt(380)
+    out = eng.beam_search(prompt, BeamParameters(num_beams=3, max_tokens=120, ignore_eos=True))
+    assert calls and {bool(k[3]) for k in eng.runner._graphs if isinstance(k, tuple)} == {False, True}
+    for h in out.hypotheses:
+        z = np.asarray(P.forward_logits(m.plain_cfg, m.W, prompt + h.tokens[:-1]), dtype=np.float64)[len(prompt) - 1:]
+        z -= z.max(1, keepdims=True)
+        want = float((z[np.arange(120), h.tokens] - np.log(np.exp(z).sum(1))).sum())
+        assert abs(h.score - want) <= 120 * 5e-7 + 2e-5

@@ -319,3 +319,76 @@ def test_a_beams_score_goes_to_the_device_in_two_parts():
     (a, b, none), = BeamSearch._candidates(chosen)
     assert a[1:] == (1, 7) and b[1:] == (0, 3) and none == (-math.inf, -1, -1)
     assert abs(a[0] - scores[0]) <= 2.0 ** -48 * abs(scores[0]) and abs(b[0] - scores[2]) <= 2.0 ** -48
+
+
+# Both kernels' times on the card, us: (dtype, requests, beams, heads, key heads, head size, page, positions of the table, window, positions, shared ones) ->
+# (the kernel that takes a sequence by itself, the one that reads shared pages once).
+MEASURED = [
+    (("bfloat16", 2, 3, 4, 4, 16, 64, 2048, 0, 23, 0), (6.5, 7.5)),
+    (("bfloat16", 8, 4, 4, 4, 16, 32, 1024, 0, 40, 0), (4.1, 7.4)),
+    (("bfloat16", 1, 3, 32, 8, 128, 16, 1024, 0, 102, 32), (5.0, 9.4)),
+    (("bfloat16", 8, 5, 8, 1, 64, 16, 4096, 0, 23, 0), (4.7, 9.0)),
+    (("bfloat16", 1, 4, 12, 12, 64, 16, 1024, 0, 531, 512), (5.4, 7.8)),
+    (("bfloat16", 2, 3, 28, 4, 128, 64, 1024, 64, 76, 0), (5.4, 10.4)),
+    (("bfloat16", 4, 32, 25, 25, 64, 64, 512, 0, 393, 304), (37.8, 23.3)),
+    (("bfloat16", 8, 8, 25, 25, 64, 16, 1024, 0, 1000, 976), (53.8, 17.7)),
+    (("bfloat16", 1, 32, 32, 32, 128, 16, 13568, 0, 13566, 13552), (382.1, 59.1)),
+    (("bfloat16", 16, 2, 28, 4, 128, 16, 2048, 0, 601, 590), (33.9, 12.5)),
+    (("float32", 1, 32, 4, 4, 32, 32, 1024, 0, 24, 0), (5.0, 7.9)),
+    (("float32", 1, 4, 2, 2, 48, 64, 1024, 0, 33, 0), (5.1, 10.4)),
+    (("float32", 1, 8, 8, 8, 128, 16, 2048, 64, 1256, 624), (7.9, 14.8)),
+    (("float32", 2, 32, 6, 3, 64, 16, 8192, 0, 33, 24), (7.5, 11.7)),
+    (("float32", 2, 4, 28, 4, 128, 16, 2048, 0, 843, 400), (30.9, 19.1)),
+    (("float32", 1, 16, 32, 32, 128, 32, 32768, 0, 3785, 3712), (206.0, 41.4)),
+]
+
+
+@pytest.fixture
+def beams_library():
+    from deliverance_amd.kernels import build
+    try:
+        build.build(only=["attn_beams", "attn_f32", "run_step"], verbose=False)
+    except build.KernelLibraryError as e:
+        pytest.skip(str(e))
+
+
+@pytest.mark.parametrize("case,times", MEASURED)
+def test_steps_of_beams_go_to_the_faster_kernel(case, times, beams_library):
+    import torch
+    from deliverance_amd.kernels import ops
+    dtype, groups, beams, heads, kv_heads, dim, page, width, window, length, shared = case
+    gone = max(0, length - window) if window else 0
+    here = ops.attention_beams_pays(groups, beams, heads, kv_heads, dim, page, width // page, getattr(torch, dtype), length - gone, max(0, shared - gone))
+    assert here == (times[1] < times[0])
+
+
+def test_what_a_step_of_beams_is_judged_by(beams_library, monkeypatch):
+    """Positions that a window has left behind are neither seen nor shared; a step that would leave the calls issued from C++ has to be worth it."""
+    from types import SimpleNamespace as N
+    import torch
+    from deliverance_amd.engine.step import BeamStep, StepRunner
+    from deliverance_amd.kernels import ops
+    layers = [N(mixer=N(paged_attention=lambda w=w: ((0, 4, 2, 64, w),))) for w in (0, 50)]
+    runner = N(model=N(blocks=layers, dtype=torch.bfloat16, config=N(schedule=[N(cache=0, layer=0), N(cache=1, layer=1), N(cache=0, layer=0)])),
+               cache=N(group_of_slot={0: 0, 1: 1}, page_size=16), native=object(), debug_hook=None, _beam_layers=None, PART_BY_PART_US=46.0)
+    asked = []
+    monkeypatch.setattr(ops, "attention_beams_pays", lambda *a, host_us=0.0: (asked.append((a[-2:], host_us)), a[-1] > 0)[1])
+    step = BeamStep(2, 4, [0.0] * 4, [[64, 96], [64, 96]])
+    attend = StepRunner._beams_attend(runner, step, [70, 70, 110, 110], 8, 16, recorded=True)
+    assert asked == [((90, 80), 0.0), ((50, 40), 0.0)] and attend == {(0, 4, 2, 64, 0), (1, 4, 2, 64, 50)}
+    asked.clear()
+    attend = StepRunner._beams_attend(runner, BeamStep(2, 4, [0.0] * 4, [[0, 0], [16, 16]]), [70, 70, 110, 110], 4, 16, recorded=False)
+    assert asked == [((90, 0), 46.0), ((50, 0), 46.0)] and attend == frozenset()
+    assert StepRunner._beams_attend(runner, BeamStep(1, 4, [0.0] * 2, [[64, 64], [64, 64]]), [70, 70], 2, 16, recorded=True) == frozenset()
+
+
+def test_the_estimate_of_unusual_steps(beams_library):
+    """Whatever the sizes, an answer; what cannot be is behind."""
+    from deliverance_amd.kernels import ops
+    ahead = ops._lib().da_attn_beams_ahead_ns
+    big = ahead(1023, 64, 32, 32, 256, ops.BF16, 2 ** 20, 16, 1, 1, 2 ** 24, 2 ** 24)
+    assert big == 10 ** 9
+    for bad in ((0, 4, 4, 4, 64, ops.BF16, 8, 16, 1, 1, 10, 0), (1, 4, 4, 0, 64, ops.BF16, 8, 16, 1, 1, 10, 0), (1, 4, 4, 4, 60, ops.BF16, 8, 16, 1, 1, 10, 0),
+                (1, 4, 4, 4, 64, ops.BF16, 8, 16, 1, 0, 10, 0), (1, 4, 4, 4, 64, ops.BF16, 8, 16, 1, 1, 0, 0)):
+        assert ahead(*bad) == -1
+    assert abs(ahead(1, 4, 4, 4, 64, ops.BF16, 8, 16, 1, 1, 10, -5)) < 10 ** 5 and abs(ahead(1, 4, 4, 4, 64, ops.F32, 8, 16, 1, 1, 10, 50)) < 10 ** 5
