@@ -435,26 +435,48 @@ class StepRunner:
         return ctx
 
     # ---- decode-only steps replayed from a HIP graph ----------------------------------------------
+    # Recordings of beam search's steps that are kept, with their scratch buffers: those that were used last.  (A search whose prompts end one after another
+    # and that goes over to the other attention has two for each power of two of requests.)
+    MAX_BEAM_RECORDINGS = 16
+
+    @staticmethod
+    def _bucket(n: int) -> int:
+        return 1 << (n - 1).bit_length()
+
+    def _beam_bucket(self, n_seqs: int, n_beams: int) -> int:
+        """Beams are padded request by request, to no more of them than the engine takes."""
+        return min(self._bucket(n_seqs // n_beams), max(n_seqs, self.max_graph_batch) // n_beams) * n_beams
+
+    def _keep_recording(self, key) -> None:
+        """The recording (or the one that is about to be made) was used last; the one that was not for the longest time goes."""
+        if key in self._graphs:
+            self._graphs[key] = self._graphs.pop(key)
+            return
+        of_beams = [k for k in self._graphs if isinstance(k, tuple)]
+        if len(of_beams) >= self.MAX_BEAM_RECORDINGS:
+            torch.cuda.synchronize()                       # (its last replay may be under way)
+            del self._graphs[of_beams[0]]
+
     def _run_graph(self, entries, starts, sample_records, beams=None):
         """A step of one-token sequences only has a fixed shape once it is padded to a bucket
         size, so its kernels (model and sampling, or the choice among beams) are recorded once per bucket and
         replayed.  Only the step's integers change: they are copied into the bucket's own buffer first."""
         from ..kernels import ops
         S = len(entries)
-        unit = 1 if beams is None else beams.n_beams       # (beams are padded request by request)
-        bucket = unit
-        while bucket < S:
-            bucket *= 2
+        bucket = self._bucket(S) if beams is None else self._beam_bucket(S, beams.n_beams)
         order = list(range(S))
         extra, a_pad = sample_records, RECORD_WORDS
         if beams is not None:
-            extra, a_pad = self._beam_words(beams, bucket // unit) + self._beam_low_words(beams, bucket // unit), 0
+            n = bucket // beams.n_beams
+            extra, a_pad = self._beam_words(beams, n) + self._beam_low_words(beams, n), 0
         offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap, extra=extra, extra_a_pad=a_pad)
         key, attend = bucket, None
         if beams is not None:                              # (a step's kernels are recorded: which attention they hold is part of its name)
             attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries], bucket, self.max_blocks_cap, recorded=True)
             key = (bucket, beams.n_beams, beams.n_keep, attend)
         st = self._graphs.get(key)
+        if beams is not None:
+            self._keep_recording(key)
         if st is None:
             host = torch.empty(n_words, dtype=torch.int32, pin_memory=True)
             st = {"dev": torch.empty(n_words, dtype=torch.int32, device=self.device),
@@ -498,5 +520,5 @@ class StepRunner:
         if beams is None:
             ctx.sampled = sampled[:S]
         else:
-            ctx.chosen = st["chosen"][:, :S // unit]
+            ctx.chosen = st["chosen"][:, :S // beams.n_beams]
         return st["logits"][:S], ctx

@@ -110,3 +110,22 @@ def test_a_search_takes_the_kernel_that_its_positions_pay_for(tmp_path, monkeypa
         z -= z.max(1, keepdims=True)
         want = float((z[np.arange(120), h.tokens] - np.log(np.exp(z).sum(1))).sum())
         assert abs(h.score - want) <= 120 * 5e-7 + 2e-5
+
+
+@pytest.mark.needs_device
+def test_searches_of_many_kinds_keep_few_recordings(models):
+    """One engine, searches of many numbers of beams and prompts, and the first of them again when its recording has gone."""
+    from deliverance_amd import AutoModelForCausalLM, BeamParameters, GeneratorParameters
+    m = models["A"]
+    eng = AutoModelForCausalLM.from_pretrained(m.folder, dtype="float32", max_cached_tokens=2048, max_num_seqs=15)
+    eng.runner.MAX_BEAM_RECORDINGS = 3
+    greedy = eng.generate(m.prompt(5), GeneratorParameters(max_tokens=4, ignore_eos=True)).generated_tokens
+    prompts = [m.prompt(n) for n in (5, 9, 17)]
+    found = {}
+    for beams, n in ((4, 1), (2, 2), (3, 3), (5, 3), (2, 1), (4, 1), (5, 3), (1, 3)):
+        out = eng.beam_search(prompts[:n], BeamParameters(num_beams=beams, max_tokens=6, ignore_eos=True))
+        for k, r in enumerate(out):
+            assert found.setdefault((beams, k), [h.tokens for h in r.hypotheses]) == [h.tokens for h in r.hypotheses]
+        keys = [k for k in eng.runner._graphs if isinstance(k, tuple)]
+        assert len(keys) <= 3 and all(k[0] <= 15 for k in keys)
+    assert eng.generate(m.prompt(5), GeneratorParameters(max_tokens=4, ignore_eos=True)).generated_tokens == greedy

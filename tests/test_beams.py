@@ -321,6 +321,30 @@ def test_a_beams_score_goes_to_the_device_in_two_parts():
     assert abs(a[0] - scores[0]) <= 2.0 ** -48 * abs(scores[0]) and abs(b[0] - scores[2]) <= 2.0 ** -48
 
 
+def test_a_step_of_beams_is_padded_to_no_more_than_the_engine_takes():
+    from types import SimpleNamespace as N
+    from deliverance_amd.engine.step import StepRunner
+    runner = N(max_graph_batch=64, _bucket=StepRunner._bucket)
+    pad = lambda n, b: StepRunner._beam_bucket(runner, n * b, b)  # noqa: E731
+    assert [pad(n, 7) for n in (1, 2, 3, 5, 9)] == [7, 14, 28, 56, 63]         # (nine requests of seven beams: 63 rows, not 112)
+    assert [pad(n, 1) for n in (1, 3, 64)] == [1, 4, 64] and pad(1, 64) == 64 and pad(2, 33) == 66
+    assert [StepRunner._bucket(n) for n in (1, 2, 3, 4, 5, 64, 65)] == [1, 2, 4, 4, 8, 64, 128]
+
+
+def test_recordings_of_steps_of_beams_do_not_pile_up(monkeypatch):
+    from types import SimpleNamespace as N
+    import torch
+    from deliverance_amd.engine.step import StepRunner
+    waits = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: waits.append(1))
+    runner = N(MAX_BEAM_RECORDINGS=2, _graphs={8: "sampled"})
+    for key in ((4, 4), (8, 4), (4, 4), (6, 3), (4, 4)):
+        StepRunner._keep_recording(runner, key)
+        runner._graphs.setdefault(key, "recording")
+    assert list(runner._graphs) == [8, (6, 3), (4, 4)] and waits == [1]
+    assert StepRunner.MAX_BEAM_RECORDINGS >= 8
+
+
 # Both kernels' times on the card, us: (dtype, requests, beams, heads, key heads, head size, page, positions of the table, window, positions, shared ones) ->
 # (the kernel that takes a sequence by itself, the one that reads shared pages once).
 MEASURED = [
