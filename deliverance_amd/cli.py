@@ -52,6 +52,9 @@ def cmd_generate(a) -> int:
     if a.num_beams is not None and (a.temperature or any(v is not None for v in (a.top_k, a.top_p, a.uniform_top_p, a.xtc_threshold, a.xtc_probability))):
         print("--num-beams searches for the most likely tokens: it takes no temperature and no filters", file=sys.stderr)
         return 2
+    if a.num_beams is None and (a.length_penalty is not None or a.early_stopping):
+        print("--length-penalty and --early-stopping belong to beam search: give --num-beams", file=sys.stderr)
+        return 2
     cfg = {}
     if a.model_config:
         with open(a.model_config) as f:
@@ -117,8 +120,8 @@ def _print_profile(a) -> None:
 def _beam_search(a, model, prompts) -> int:
     """The best hypothesis of every prompt on stdout, all of them in the JSONL file."""
     from .engine.beams import BeamParameters
-    params = BeamParameters(num_beams=a.num_beams, max_tokens=a.max_tokens, ntokens=a.ntokens, length_penalty=a.length_penalty,
-                            early_stopping=a.early_stopping, ignore_eos=a.ignore_eos)
+    params = BeamParameters(num_beams=a.num_beams, max_tokens=a.max_tokens, ntokens=a.ntokens,
+                            length_penalty=1.0 if a.length_penalty is None else a.length_penalty, early_stopping=a.early_stopping, ignore_eos=a.ignore_eos)
     from .profiler import InferenceProfiler, KernelProfiler
     for p in prompts[:a.warmup_cases]:
         model.beam_search(p, params)
@@ -205,7 +208,7 @@ def main(argv=None) -> int:
     g.add_argument("--xtc-probability", type=float, default=None)
     g.add_argument("--ignore-eos", action="store_true")
     g.add_argument("--num-beams", type=int, default=None, help="beam search with so many beams in place of sampling")
-    g.add_argument("--length-penalty", type=float, default=1.0, help="beam search: hypotheses are ranked by score / length ** this, default 1.0")
+    g.add_argument("--length-penalty", type=float, default=None, help="beam search: hypotheses are ranked by score / length ** this, default 1.0")
     g.add_argument("--early-stopping", action="store_true", help="beam search: a prompt ends with its first num-beams finished hypotheses")
     g.add_argument("--warmup-cases", type=int, default=1, help="prompts to run before recording, default 1")
     g.add_argument("--max-cases", type=int, default=None)
@@ -216,7 +219,7 @@ def main(argv=None) -> int:
     g.add_argument("--model-config", help="JSON file with engine settings (EngineConfig fields)")
     g.add_argument("--no-batch", dest="batch", action="store_false", help="one request at a time, as the reference runs them")
     g.add_argument("--profile-stages", action="store_true")
-    g.add_argument("--output", help="CSV: prompt_tokens,generated_tokens,total_ms,generation_ms,tokens_per_second")
+    g.add_argument("--output", help="CSV: prompt_tokens,generated_tokens,total_ms,generation_ms,tokens_per_second (beam search: the first three)")
     g.add_argument("--jsonl-output")
     g.set_defaults(fn=cmd_generate)
     r = sub.add_parser("random", help="write a model folder with seeded random weights")

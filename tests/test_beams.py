@@ -217,6 +217,13 @@ def test_the_command_line_takes_beams_or_sampling():
         assert cli.main(["generate", "--model", "/nonexistent", "--prompt-ids", "1,2", "--num-beams", "2", *more]) == 2
 
 
+def test_the_command_line_refuses_what_only_beam_search_has(capsys):
+    from deliverance_amd import cli
+    for more in (["--length-penalty", "0.5"], ["--early-stopping"]):
+        assert cli.main(["generate", "--model", "/nonexistent", "--prompt-ids", "1,2", *more]) == 2
+        assert "--num-beams" in capsys.readouterr().err
+
+
 def test_operands_on_another_device_are_refused(monkeypatch):
     import torch
     from deliverance_amd.kernels import ops
