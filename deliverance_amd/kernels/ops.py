@@ -266,6 +266,15 @@ def _dev_here(*ts):
             here = d
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _fit_int(what: str, *sizes):
+    """Sizes that the library takes as 32-bit numbers (a larger one would arrive as another)."""
+    if max(sizes) > _INT_MAX:
+        raise KernelError(f"{what}: sizes {list(sizes)} pass 32 bits")
+
+
 def _rows_2d(t: torch.Tensor, name: str):
     if not (t.dim() == 2 and t.stride(1) == 1):
         raise KernelError(f"{name} must be 2-D with a contiguous last dimension")
@@ -377,6 +386,7 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
     if n == 0:
         return tensors
     pool = tensors[0].shape[dim] if tensors[0].dim() > dim else -1
+    _fit_int("state_reorder", G, pool)
     table, spans = [], []
     for i, t in enumerate(tensors):
         if t.dim() <= dim or t.shape[dim] != pool or not t.is_contiguous():
@@ -855,6 +865,7 @@ MAX_BEAMS, MAX_CANDIDATES = 64, 128     # of a group (csrc/beam_select.hip)
 
 def beam_select_floats(n_rows: int, n_beams: int, vocab: int) -> int:
     """32-bit words of scratch that ``beam_select`` needs for logits [n_rows, vocab] in groups of ``n_beams``."""
+    _fit_int("beam_select", n_rows, vocab)
     n = int(_lib().da_beam_select_words(int(n_rows) // max(1, int(n_beams)), int(n_beams), int(vocab)))
     _need(n >= 0, f"beam_select: {n_rows} rows of {vocab} logits in groups of {n_beams}")
     return n
@@ -889,6 +900,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
             raise KernelError(f"beam_select: outputs must be contiguous {list(shape)}, float32 scores and int32 parents and tokens")
     if workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise KernelError("beam_select: the workspace must be contiguous float32")
+    _fit_int("beam_select", R, V)
     G, K = shape
     with _timed("beam_select", 4 * R * V, 4 * R * V, "fp32"):
         _check(_lib().da_beam_select_low(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), _ptr(scores_low), K, _ptr(out_scores),
@@ -1385,8 +1397,10 @@ def attention_beams(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torc
         raise KernelError("attention_beams: contiguous int32 block_table [S, max_blocks], seq_lens [S] and shared [S / n_beams] are needed")
     if n_splits > 1 and (workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous()):
         raise KernelError("attention_beams: more than one share needs a contiguous float32 workspace")
-    _check(_lib().da_attn_beams(_ptr(q), q.stride(0), _ptr(cache_slot), _dt(q), _ptr(block_table), block_table.shape[1], _ptr(seq_lens),
-                                _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), int(window or 0), _ptr(out), out.stride(0),
+    q_ld, out_ld = (q.stride(0), out.stride(0)) if S > 1 else (rows[1], rows[1])      # (of one row: how far the next would be does not matter)
+    _fit_int("attention_beams", S, q_ld, out_ld, block_table.shape[1], n_splits)
+    _check(_lib().da_attn_beams(_ptr(q), q_ld, _ptr(cache_slot), _dt(q), _ptr(block_table), block_table.shape[1], _ptr(seq_lens),
+                                _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), min(int(window or 0), _INT_MAX), _ptr(out), out_ld,
                                 max(1, int(n_splits)), _ptr(workspace) if n_splits > 1 else None, workspace.numel() if n_splits > 1 else 0,
                                 _stream()))
     return out

@@ -224,6 +224,46 @@ def test_the_command_line_refuses_what_only_beam_search_has(capsys):
         assert "--num-beams" in capsys.readouterr().err
 
 
+def test_sizes_beyond_32_bits_do_not_wrap(monkeypatch):
+    """The library takes sizes as 32-bit numbers: what passes them is refused, and a window that passes them sees everything."""
+    import torch
+    from deliverance_amd.kernels import ops
+    called = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: (called.append((name, a)), 0)[1]
+    monkeypatch.setattr(ops, "_lib", lambda: Library())
+    monkeypatch.setattr(ops, "_dev_here", lambda *t: None)
+    monkeypatch.setattr(ops, "_ptr", lambda t: 16)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    far = 2 ** 32
+    i32 = lambda *s: empty(*s, dtype=torch.int32)  # noqa: E731
+    f32 = lambda *s: empty(*s, dtype=torch.float32)  # noqa: E731
+    attend = dict(q=empty(2, 64), cache_slot=empty(5, 2, 1, 16, 32), block_table=i32(2, 4), seq_lens=i32(2), shared=i32(1), n_beams=2, n_heads=2, scale=1.0,
+                  window=None, out=empty(2, 64))
+    ops.attention_beams(**{**attend, "window": far + 5})
+    assert called.pop()[1][15] == 2 ** 31 - 1
+    one = dict(attend, q=empty(1, far)[:, :64], seq_lens=i32(1), block_table=i32(1, 4), n_beams=1, out=empty(1, far)[:, :64])
+    ops.attention_beams(**one)                               # (one row: how far the next would be does not matter)
+    assert called.pop()[1][1] == 64
+    for bad in (dict(q=empty(2, far)[:, :64]), dict(out=empty(2, far + 64)[:, :64]), dict(block_table=i32(2, far + 1))):
+        with pytest.raises(ops.KernelError, match="32 bits"):
+            ops.attention_beams(**{**attend, **bad})
+    out = (f32(1, 4), i32(1, 4), i32(1, 4))
+    with pytest.raises(ops.KernelError, match="32 bits"):
+        ops.beam_select(f32(2, far + 5), f32(2), 2, *out, f32(99))
+    with pytest.raises(ops.KernelError, match="32 bits"):
+        ops.beam_select_floats(2, 2, far + 5)
+    with pytest.raises(ops.KernelError, match="32 bits"):
+        ops.state_reorder([empty(far + 5, 1)], i32(1, 2), i32(1, 2))
+    assert not called
+
+
 def test_operands_on_another_device_are_refused(monkeypatch):
     import torch
     from deliverance_amd.kernels import ops
