@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from deliverance_amd.kernels import ops
-from test_beams_gpu import DEV, attend, beams_case, quick
+from test_beams_gpu import DEV, attend, beams_case, check_attention, check_select, quick
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,47 @@ def test_weights_keep_their_32_bits(length, shared, dtype):
     got = attend(c).cpu().double()
     near = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -22
     assert bool(((got - want).abs() <= near).all()), ((got - want).abs() / near).max()
+
+
+# Calls that reach what smaller ones do not: four loads of logits a wavefront (from 16,384 loads on) with long and with short segments, four segments' keys a
+# thread (from 2,049 segments a group on), segments past the kept ones (from 4,097), segments numbered by a division (from 65,536).
+@pytest.mark.parametrize("groups,beams,vocab,keep", [(32, 8, 131071, 16), (1, 8, 140000, 128), (600, 1, 7000, 12), (1, 64, 262145, 40), (3, 5, 262143, 10)])
+def test_choices_among_many_logits(groups, beams, vocab, keep):
+    g = torch.Generator().manual_seed(groups + vocab)
+    logits = torch.randn(groups * beams, vocab, generator=g) * 3
+    logits[:, 17::29] = -math.inf
+    scores = -20 * torch.rand(groups * beams, generator=g)
+    if beams > 2:
+        scores[beams - 1::beams] = -math.inf
+    check_select(logits.to(DEV), scores.to(DEV), beams, keep)
+
+
+def test_equal_entries_among_many_logits():
+    """The first ones in the order of beams and tokens, through the divisions too."""
+    logits = torch.full((64, 262145), 0.5)
+    logits[1:, 5::2] = 1.5
+    check_select(logits.to(DEV), torch.full((64,), -2.0, device=DEV), 64, 128)
+
+
+# Four wavefronts a workgroup: with more workgroups than compute units, and over many chunks, at every head size that has both forms.
+FOUR_WAVES = [(9, 4, 32, 32, 128, 16, [140 + i % 3 for i in range(36)], [128] * 9), (9, 4, 32, 32, 32, 32, [100 + i % 5 for i in range(36)], [96] * 9),
+              (10, 3, 28, 28, 64, 16, [90] * 30, [80] * 10), (9, 4, 30, 30, 80, 16, [70] * 36, [64] * 9),
+              (1, 2, 2, 1, 128, 64, [3200, 3199], [3072]), (1, 3, 2, 2, 32, 16, [3100, 3085, 3073], [3072]), (1, 2, 1, 1, 64, 32, [3090, 3074], [1024]),
+              (1, 2, 4, 2, 96, 16, [3105, 3105], [0])]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("groups,beams,heads,kv_heads,dim,page,lengths,shared", FOUR_WAVES)
+def test_attention_of_beams_by_four_wavefronts(groups, beams, heads, kv_heads, dim, page, lengths, shared, dtype):
+    c = beams_case(groups, beams, heads, kv_heads, dim, page, dtype, lengths, shared, seed=dim + beams)
+    workgroups = groups * kv_heads * -(-beams * (heads // kv_heads) // 16)
+    assert workgroups > 256 or c["table"].shape[1] * page // 64 >= 48
+    check_attention(c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_groups_of_many_beams_over_windows(dtype):
+    """Shared heads, windows that end inside shared pages and places without a beam, in one call."""
+    c = beams_case(5, 6, 12, 3, 64, 16, dtype, [300 + 7 * (i // 6) if i % 6 != 4 else 0 for i in range(30)], [288] * 5, seed=8)
+    for window in (1, 20, 64, 290):
+        check_attention(c, window=window, splits=2)

@@ -46,3 +46,14 @@ def test_the_others_do_not_spill(unit, name):
     except AssertionError:
         pytest.fail(f"{name} is not in {unit}")
     assert all(scratch == 0 and workgroups >= 1 for workgroups, scratch in found.values())
+
+
+def test_reordering_does_not_spill():
+    """A thread of the widest form keeps 64 columns; every form is compiled and has no scratch memory."""
+    try:
+        build.build(only=["reorder"], verbose=False)
+    except build.KernelLibraryError as e:
+        pytest.skip(str(e))
+    with open(build.unit_path("reorder"), "rb") as f:
+        found = {k[".name"]: k[".private_segment_fixed_size"] for elf in _code_objects(f.read()) for k in _notes(elf) if "reorder_kernel" in k[".name"]}
+    assert len(found) == 5 and not any(found.values()), found
