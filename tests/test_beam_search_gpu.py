@@ -189,3 +189,30 @@ def test_profile_of_a_beam_search(models):
                        capture_output=True, text=True, timeout=300)
     assert p.returncode == 0, p.stderr
     assert all(word in p.stderr for word in ("profile summary", "beam_search.prompts", "beam_search.step", "beam_select", "state_reorder"))
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_windows_and_grouped_heads_read_what_beams_share_once(graphs, tmp_path, monkeypatch):
+    """A design with short and long windows and several query heads a key head, recurrent mixers beside them: its attention sent to the kernel
+    that reads shared pages once whatever the estimate says, over pages that windows give back."""
+    from deliverance_amd import BeamParameters
+    from deliverance_amd.kernels import ops
+    from deliverance_amd.random_model import random_model
+    from pafolorn_models import attention, delta, parallel_layer
+    import plain_pafolorn as plain
+    cfg = {"architecture": "Pafolorn", "vocab": 300, "width": 64, "norm": {"eps": 1e-5}, "logit_scale": 0.7,
+           "layers": [parallel_layer(attention(4, 2, 32, 32, 0.18, 40, 0, 10000.0, 16), delta(4, 2, 16, 32, 4), 1.3, 0.8, ff=96),
+                      parallel_layer(attention(8, 2, 16, 16, 0.25, 4096, 0, 500.0, 16), delta(2, 2, 16, 16, 2), 1.0, 1.0)]}
+    random_model(str(tmp_path), cfg, seed=23)
+    pcfg, W = plain.read_model_folder(str(tmp_path))
+    calls, kernel = [], ops.attention_beams
+    monkeypatch.setattr(ops, "attention_beams", lambda *a, **k: (calls.append((a[6], a[8])), kernel(*a, **k))[1])
+    monkeypatch.setattr(ops, "attention_beams_pays", lambda *a, **k: True)
+    eng = load(tmp_path, use_graphs=graphs, poison_freed_pages=True)
+    prompts = [[int(t) for t in np.random.default_rng(n).integers(0, 300, size=n)] for n in (29, 101)]
+    outs = eng.beam_search(prompts, BeamParameters(num_beams=3, max_tokens=40, ignore_eos=True))
+    assert set(calls) == {(4, 40), (8, 4096)}
+    for prompt, out in zip(prompts, outs):
+        check(out, lambda ids: plain.forward_logits(pcfg, W, ids)[-1], prompt, 3, 40)
+    eng.cache.manager.check()
+    assert eng.cache.manager.live() == []
