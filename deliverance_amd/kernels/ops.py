@@ -269,10 +269,9 @@ def _dev_here(*ts):
 _INT_MAX = 2 ** 31 - 1
 
 
-def _fit_int(what: str, *sizes):
-    """Sizes that the library takes as 32-bit numbers (a larger one would arrive as another)."""
-    if max(sizes) > _INT_MAX:
-        raise KernelError(f"{what}: sizes {list(sizes)} pass 32 bits")
+def _past_int(what: str, *sizes):
+    """The library takes sizes as 32-bit numbers: a larger one would arrive as another."""
+    raise KernelError(f"{what}: one of the sizes {list(sizes)} passes 32 bits")
 
 
 def _rows_2d(t: torch.Tensor, name: str):
@@ -386,7 +385,8 @@ def state_reorder(tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents:
     if n == 0:
         return tensors
     pool = tensors[0].shape[dim] if tensors[0].dim() > dim else -1
-    _fit_int("state_reorder", G, pool)
+    if G > _INT_MAX or pool > _INT_MAX:
+        _past_int("state_reorder", G, pool)
     table, spans = [], []
     for i, t in enumerate(tensors):
         if t.dim() <= dim or t.shape[dim] != pool or not t.is_contiguous():
@@ -865,7 +865,8 @@ MAX_BEAMS, MAX_CANDIDATES = 64, 128     # of a group (csrc/beam_select.hip)
 
 def beam_select_floats(n_rows: int, n_beams: int, vocab: int) -> int:
     """32-bit words of scratch that ``beam_select`` needs for logits [n_rows, vocab] in groups of ``n_beams``."""
-    _fit_int("beam_select", n_rows, vocab)
+    if n_rows > _INT_MAX or vocab > _INT_MAX:
+        _past_int("beam_select", n_rows, vocab)
     n = int(_lib().da_beam_select_words(int(n_rows) // max(1, int(n_beams)), int(n_beams), int(vocab)))
     _need(n >= 0, f"beam_select: {n_rows} rows of {vocab} logits in groups of {n_beams}")
     return n
@@ -882,27 +883,34 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     ``workspace``: float32, ``beam_select_floats`` elements.  Sums are 64-bit inside.  Where choices follow one another, what a
     float32 score leaves of its sum goes to ``out_scores_low`` (like ``out_scores``; 0 for an infinite score) and comes back as ``scores_low``
     (like ``scores``): score + low carries 48 bits, where a score alone is rounded at the size of the whole sum with every token."""
-    _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace, scores_low, out_scores_low)
+    _dev_here(logits, scores, out_scores, out_parents, out_tokens, workspace)
     _rows_2d(logits, "logits")
     R, V = logits.shape
     if not 1 <= n_beams <= MAX_BEAMS or R % n_beams:
         raise KernelError(f"beam_select: {R} rows in groups of {n_beams} (1 to {MAX_BEAMS})")
     if logits.dtype != torch.float32 or scores.dtype != torch.float32 or scores.numel() != R or not scores.is_contiguous():
         raise KernelError("beam_select: logits and scores must be float32, one score a row")
-    if scores_low is not None and (scores_low.dtype != torch.float32 or scores_low.numel() != R or not scores_low.is_contiguous()):
-        raise KernelError("beam_select: scores_low must be float32, one a row")
     shape = (R // n_beams, out_scores.shape[-1] if out_scores.dim() else 0)
     if not 1 <= shape[1] <= MAX_CANDIDATES:
         raise KernelError(f"beam_select: {shape[1]} candidates (1 to {MAX_CANDIDATES})")
-    low = out_scores if out_scores_low is None else out_scores_low
-    for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32), (low, torch.float32)):
+    for t, dtype in ((out_scores, torch.float32), (out_parents, torch.int32), (out_tokens, torch.int32)):
         if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
             raise KernelError(f"beam_select: outputs must be contiguous {list(shape)}, float32 scores and int32 parents and tokens")
     if workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise KernelError("beam_select: the workspace must be contiguous float32")
-    _fit_int("beam_select", R, V)
+    if R > _INT_MAX or V > _INT_MAX:
+        _past_int("beam_select", R, V)
     G, K = shape
     with _timed("beam_select", 4 * R * V, 4 * R * V, "fp32"):
+        if scores_low is None and out_scores_low is None:
+            _check(_lib().da_beam_select(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), K, _ptr(out_scores), _ptr(out_parents),
+                                         _ptr(out_tokens), _ptr(workspace), workspace.numel(), _stream()))
+            return out_scores, out_parents, out_tokens
+        _dev_here(logits, scores_low, out_scores_low)
+        if scores_low is not None and (scores_low.dtype != torch.float32 or scores_low.numel() != R or not scores_low.is_contiguous()):
+            raise KernelError("beam_select: scores_low must be float32, one a row")
+        if out_scores_low is not None and (out_scores_low.dtype != torch.float32 or out_scores_low.shape != shape or not out_scores_low.is_contiguous()):
+            raise KernelError(f"beam_select: out_scores_low must be contiguous float32 {list(shape)}")
         _check(_lib().da_beam_select_low(_ptr(logits), logits.stride(0), G, n_beams, V, _ptr(scores), _ptr(scores_low), K, _ptr(out_scores),
                                          _ptr(out_scores_low), _ptr(out_parents), _ptr(out_tokens), _ptr(workspace), workspace.numel(),
                                          _stream()))
@@ -1398,9 +1406,11 @@ def attention_beams(q: torch.Tensor, cache_slot: torch.Tensor, block_table: torc
     if n_splits > 1 and (workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous()):
         raise KernelError("attention_beams: more than one share needs a contiguous float32 workspace")
     q_ld, out_ld = (q.stride(0), out.stride(0)) if S > 1 else (rows[1], rows[1])      # (of one row: how far the next would be does not matter)
-    _fit_int("attention_beams", S, q_ld, out_ld, block_table.shape[1], n_splits)
-    _check(_lib().da_attn_beams(_ptr(q), q_ld, _ptr(cache_slot), _dt(q), _ptr(block_table), block_table.shape[1], _ptr(seq_lens),
-                                _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), min(int(window or 0), _INT_MAX), _ptr(out), out_ld,
+    blocks = block_table.shape[1]
+    if S > _INT_MAX or q_ld > _INT_MAX or out_ld > _INT_MAX or blocks > _INT_MAX or n_splits > _INT_MAX:
+        _past_int("attention_beams", S, q_ld, out_ld, blocks, n_splits)
+    _check(_lib().da_attn_beams(_ptr(q), q_ld, _ptr(cache_slot), _dt(q), _ptr(block_table), blocks, _ptr(seq_lens),
+                                _ptr(shared), G, n_beams, n_heads, Hkv, D, page, float(scale), min(int(window), _INT_MAX) if window else 0, _ptr(out), out_ld,
                                 max(1, int(n_splits)), _ptr(workspace) if n_splits > 1 else None, workspace.numel() if n_splits > 1 else 0,
                                 _stream()))
     return out
