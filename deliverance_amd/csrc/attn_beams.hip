@@ -18,8 +18,9 @@
 // otherwise: with two, small differences of weights are off by more than the result's rounding, for 1 % (8 x 8 beams over 1,003 positions 17.4 us
 // in place of 17.7, 1 x 4 over 531 7.7 in place of 7.8, 4 x 4 over 32,701 the same).  32-bit: 16x16x4 products, nothing is rounded.
 // Bound by memory where contexts are long (4 x 4 beams, 32 / 8 heads of 128, 32,701 positions: 101 us, 5.4 TB/s), else by three round trips, lengths,
-// pages, keys and values, of which the second travels beside the chunk before (4 x 4 beams 124 -> 114 us; 8 x 8 of 25 heads over 1,003 positions 21.4 -> 17.4
-// with 8 wavefronts).  1 x 4 beams of 12 heads over 531 positions: 7.8 us.
+// pages, keys and values, of which the second travels beside the chunk before.  us: 1 x 4 beams of 12 heads over 531 positions 7.9, 8 x 8 of 25 heads over
+// 1,003 17.7; 32-bit, 2 x 5 of 12 heads over 777 10.2 and the joining kernel's 3.1: there a share has too few chunks for 8 wavefronts, and each loads its two
+// halves one after the other (the products are a sixth of the time).
 #include "gemm_common.h"
 #include <da_lane_swap.h>
 
@@ -436,9 +437,10 @@ extern "C" int da_attn_beams_splits(int G, int B, int Hq, int Hkv, int D, int dt
   return n < 1 ? 1 : (n > DA_WAVE ? DA_WAVE : (int)n);
 }
 
-// Wavefronts of a workgroup.  8 where there is one workgroup a compute unit, which they fill by themselves: 8 x 8 beams of 25 heads over 1,003 positions
-// 17.3 us for 20.1, 24 beams of 7 heads over 3,456 11.5 for 13.6.  4 where more share one, and where each has so many chunks that 4 wavefronts
-// keep the memory busy: 4 x 4 beams over 32,701 positions, 64 chunks each, 104 us for 113 (26 chunks each: 29.2 for 27.5).
+// Wavefronts of a workgroup.  8 where there is one workgroup a compute unit, which they fill by themselves (us a call in a chain, 8 / 4): 8 x 8 beams of 25 heads
+// over 1,003 positions 18.1 / 21.1, 1 x 4 of 12 heads over 531 8.0 / 9.1, 24 beams of 7 heads over 3,456 11.7 / 11.9.  4 where more share one, and where each has so
+// many chunks that 4 wavefronts keep the memory busy: 4 x 4 beams of 32 / 8 heads of 128 over 32,701 positions, 64 chunks each, 116 / 108.  26 chunks
+// each lie between: heads of 64 29.0 / 30.4, 26.7 / 28.9, 25.7 / 27.0, of 128 53.9 / 52.4, 68.6 / 71.6.
 static int beam_waves(long groups, int splits, int max_blocks, int page) {
   return groups * splits > 256 || (long)max_blocks * page / CHUNK >= 48L * splits ? 4 : 8;
 }

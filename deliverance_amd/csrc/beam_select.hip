@@ -17,8 +17,10 @@
 // segments reach it).  It reads the segments that reach it again; the entries that do are cut down by bounds of the same
 // kind until they are few, and put in order by counting, for each, those in front of it.  A bound is a key and a place, so that equal logits
 // are cut down too; where more entries reach the first one than the list holds, it is searched bit by bit.
-// us, first and second kernel: 32 x 8 beams, vocabulary 131,071 26.3 (5.1 TB/s) and 9.7; 8 x 8, 50,257 5.6 and 8.0; 1 x 4 2.7 and 6.3.  The second is a chain
+// us, first and second kernel: 32 x 8 beams, vocabulary 131,071 26.2 (5.1 TB/s) and 9.6; 8 x 8, 50,257 5.5 and 8.0; 1 x 4 2.6 and 6.3.  The second is a chain
 // of eight barriers and three round trips to memory in one workgroup a group, whatever the logits (one beam far ahead, all equal, in order: within 8 us of it).
+// Above 32 candidates the groups of threads are smaller, and each thread counts more of them: both kernels, 50,257, 1 x 16 beams and 32 candidates 14.0,
+// 1 x 32 and 64 21.9, 4 x 32 and 64 27.0, 1 x 64 and 128 42.1.
 #include "common.h"
 
 #define BEAM_MAX 64              // beams of a group

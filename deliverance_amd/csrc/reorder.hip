@@ -8,7 +8,8 @@
 //
 // Bound by memory: every row that moves is read and written once.  Loads and stores go past the caches: 8 x 8 beams' pages of 48
 // layers of 25 heads, 315 MB, take 62.9 us (5.0 TB/s, a large copy 5.13) and 98 with ordinary ones, states of 543 MB 112 and
-// 207; two columns a thread are behind (64.9, 117).
+// 207; two columns a thread are behind (64.9, 117).  Above 16 places a column is 4 bytes, at the same rate (2 x 32 places of those pages 58.9 us, 1 x 64 60.9);
+// rows of an odd number of 2-byte units go by those (8 x 8 places 421, 2 x 32 198).
 #include "common.h"
 #include <da_anew.h>
 

@@ -3,8 +3,9 @@
 Every prompt has ``num_beams`` beams, each a request of the cache manager.  A step runs one token of every beam of every prompt;
 ``ops.beam_select`` chooses among all beams and the vocabulary; a beam that is continued keeps its place, the places of the others
 go to what continues it: the cache manager shares the full pages (``CacheManager.reorder``) and ``ops.state_reorder`` copies
-what a beam holds for itself, the page that is being written and its recurrent states.  In attention over all keys the pages that
-a prompt's beams have in common are read once for all of them (``ops.attention_beams``).
+what a beam holds for itself, the page that is being written and its recurrent states.  Layers of softmax attention without extras (those that go
+through ``ops.paged_attention``) read the pages that a prompt's beams have in common once for all of them where that is ahead (``ops.attention_beams``);
+the other designs' attention and latent rows are read beam by beam.
 
 ``BeamGroup`` is the host's part of the search for one prompt and sees candidates only; ``BeamSearch`` drives the engine.
 """
