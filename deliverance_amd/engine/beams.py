@@ -16,6 +16,7 @@ import time
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ..kernels import ops
@@ -259,8 +260,8 @@ class BeamSearch:
     @staticmethod
     def _candidates(chosen: torch.Tensor) -> List[List[Tuple[float, int, int]]]:
         """(score, parent, token) of every place; a score is the sum of its two 32-bit parts."""
-        scores, parents, tokens, low = chosen.cpu()
-        scores = scores.contiguous().view(torch.float32).double() + low.contiguous().view(torch.float32).double()
+        scores, parents, tokens, low = chosen.cpu().numpy()
+        scores = scores.view(np.float32).astype(np.float64) + low.view(np.float32)
         return [list(zip(s, p, t)) for s, p, t in zip(scores.tolist(), parents.tolist(), tokens.tolist())]
 
     def _advance(self, live: List[_Live]) -> None:

@@ -172,6 +172,7 @@ class StepRunner:
         self.native = NativeStep(model, cache) if native_step and self.joins_shares else None
         # (cache group, heads, key heads, head size, window) of the layers whose beams' shared pages can be read once
         self._beam_layers: Optional[List[tuple]] = None
+        self._beam_choices = {}                      # what was estimated for steps of one shape and context (see _beams_attend)
         # hook(layer, stage, tensor) for named intermediates of every step; steps then run kernel by
         # kernel, never from a recorded graph
         self.debug_hook = None
@@ -363,7 +364,7 @@ class StepRunner:
         ctx = self._context(dev, offs, meta, self.arena)
         if beams is not None:
             self._take_beams(ctx, beams)
-            ctx.beams_attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries], meta["S"], meta["max_blocks"], recorded=False)
+            ctx.beams_attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries[::beams.n_beams]], meta["S"], meta["max_blocks"], recorded=False)
         ctx.debug_hook = self.debug_hook
         self.last_ctx = ctx
         R = meta["R"]
@@ -388,7 +389,7 @@ class StepRunner:
 
     def _beams_attend(self, beams: BeamStep, lens: Sequence[int], n_seqs: int, max_blocks: int, recorded: bool) -> frozenset:
         """The layers (``StepContext.beams_attend``) of a step of ``n_seqs`` sequences in tables of ``max_blocks`` pages whose attention reads
-        what beams share once, by what the entries (of ``lens`` positions) see and share.  (The calls that are issued from C++ do not
+        what beams share once, by what its requests (of ``lens`` positions) see and share.  (The calls that are issued from C++ do not
         know of it: a step that is not recorded leaves them only for more than that costs the host.)"""
         from ..kernels import ops
         from ..profiler import KernelProfiler
@@ -399,16 +400,25 @@ class StepRunner:
                      for k, *rest in self.model.blocks[c.layer].mixer.paged_attention()]
             self._beam_layers = sorted(set(found))
         native = self.native is not None and not recorded and self.debug_hook is None and not KernelProfiler.enabled
-        lens = list(lens)[::beams.n_beams]                   # (a request's beams have one length)
-        attend = set()
-        for group, n_heads, n_kv_heads, head_dim, window in self._beam_layers:
-            gone = [max(0, n - window) if window else 0 for n in lens]
-            visible = sum(n - g for n, g in zip(lens, gone)) // len(lens)
-            shared = sum(max(0, s - g) for s, g in zip(beams.shared[group], gone)) // len(lens)
-            if ops.attention_beams_pays(n_seqs // beams.n_beams, beams.n_beams, n_heads, n_kv_heads, head_dim, self.cache.page_size, max_blocks,
-                                        self.model.dtype, visible, shared, host_us=self.PART_BY_PART_US if native else 0.0):
-                attend.add((group, n_heads, n_kv_heads, head_dim, window))
-        return frozenset(attend)
+        n, seen = len(lens), []
+        for group, _, _, _, window in self._beam_layers:
+            shared = beams.shared[group]
+            if window:
+                gone = [max(0, m - window) for m in lens]
+                seen.append((sum(min(m, window) for m in lens) // n, sum(max(0, s - g) for s, g in zip(shared, gone)) // n))
+            else:
+                seen.append((sum(lens) // n, sum(shared) // n))
+        # (estimated once for contexts that are alike, of the next 16 positions: an estimate takes the host 12 us)
+        key = (n_seqs, beams.n_beams, max_blocks, native, tuple((v // 16, s // 16) for v, s in seen))
+        attend = self._beam_choices.get(key)
+        if attend is None:
+            attend = frozenset(layer for layer, (v, s) in zip(self._beam_layers, key[4]) if ops.attention_beams_pays(
+                n_seqs // beams.n_beams, beams.n_beams, *layer[1:4], self.cache.page_size, max_blocks, self.model.dtype, 16 * v + 15, 16 * s,
+                host_us=self.PART_BY_PART_US if native else 0.0))
+            if len(self._beam_choices) >= 4096:
+                self._beam_choices.clear()
+            self._beam_choices[key] = attend
+        return attend
 
     def _context(self, dev, offs, meta, arena) -> StepContext:
         def view(name):
@@ -472,7 +482,7 @@ class StepRunner:
         offs, meta, n_words = self._layout(entries, order, pad_to=bucket, max_blocks=self.max_blocks_cap, extra=extra, extra_a_pad=a_pad)
         key, attend = bucket, None
         if beams is not None:                              # (a step's kernels are recorded: which attention they hold is part of its name)
-            attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries], bucket, self.max_blocks_cap, recorded=True)
+            attend = self._beams_attend(beams, [starts[e.rid] + 1 for e in entries[::beams.n_beams]], bucket, self.max_blocks_cap, recorded=True)
             key = (bucket, beams.n_beams, beams.n_keep, attend)
         st = self._graphs.get(key)
         if beams is not None:
@@ -493,8 +503,9 @@ class StepRunner:
         ctx = self._context(st["dev"], offs, meta, st["arena"])
         self.last_ctx = ctx
         if beams is not None:
-            self._take_beams(ctx, beams)
             ctx.beams_attend = attend
+            if st["graph"] is None:                        # (a recorded step knows where they lie)
+                self._take_beams(ctx, beams)
 
         sampled = self.sampled[:bucket]
 

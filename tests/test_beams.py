@@ -441,15 +441,18 @@ def test_what_a_step_of_beams_is_judged_by(beams_library, monkeypatch):
     from deliverance_amd.kernels import ops
     layers = [N(mixer=N(paged_attention=lambda w=w: ((0, 4, 2, 64, w),))) for w in (0, 50)]
     runner = N(model=N(blocks=layers, dtype=torch.bfloat16, config=N(schedule=[N(cache=0, layer=0), N(cache=1, layer=1), N(cache=0, layer=0)])),
-               cache=N(group_of_slot={0: 0, 1: 1}, page_size=16), native=object(), debug_hook=None, _beam_layers=None, PART_BY_PART_US=46.0)
+               cache=N(group_of_slot={0: 0, 1: 1}, page_size=16), native=object(), debug_hook=None, _beam_layers=None, _beam_choices={}, PART_BY_PART_US=46.0)
     asked = []
     monkeypatch.setattr(ops, "attention_beams_pays", lambda *a, host_us=0.0: (asked.append((a[-2:], host_us)), a[-1] > 0)[1])
     step = BeamStep(2, 4, [0.0] * 4, [[64, 96], [64, 96]])
-    attend = StepRunner._beams_attend(runner, step, [70, 70, 110, 110], 8, 16, recorded=True)
-    assert asked == [((90, 80), 0.0), ((50, 40), 0.0)] and attend == {(0, 4, 2, 64, 0), (1, 4, 2, 64, 50)}
+    attend = StepRunner._beams_attend(runner, step, [70, 110], 8, 16, recorded=True)
+    both = {(0, 4, 2, 64, 0), (1, 4, 2, 64, 50)}             # 90 and 50 positions, 80 and 40 of them shared, by steps of 16
+    assert asked == [((95, 80), 0.0), ((63, 32), 0.0)] and attend == both
+    assert StepRunner._beams_attend(runner, step, [71, 111], 8, 16, recorded=True) == both and len(asked) == 2
+    assert StepRunner._beams_attend(runner, step, [79, 119], 8, 16, recorded=True) == both and asked[2:] == [((111, 80), 0.0), ((63, 16), 0.0)]
     asked.clear()
-    attend = StepRunner._beams_attend(runner, BeamStep(2, 4, [0.0] * 4, [[0, 0], [16, 16]]), [70, 70, 110, 110], 4, 16, recorded=False)
-    assert asked == [((90, 0), 46.0), ((50, 0), 46.0)] and attend == frozenset()
+    attend = StepRunner._beams_attend(runner, BeamStep(2, 4, [0.0] * 4, [[0, 0], [16, 16]]), [70, 110], 4, 16, recorded=False)
+    assert asked == [((95, 0), 46.0), ((63, 0), 46.0)] and attend == frozenset()
     assert StepRunner._beams_attend(runner, BeamStep(1, 4, [0.0] * 2, [[64, 64], [64, 64]]), [70, 70], 2, 16, recorded=True) == frozenset()
 
 
