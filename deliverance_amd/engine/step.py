@@ -397,7 +397,7 @@ class StepRunner:
             return frozenset()
         if self._beam_layers is None:
             found = [(self.cache.group_of_slot[c.cache + k], *rest) for c in self.model.config.schedule
-                     for k, *rest in self.model.blocks[c.layer].mixer.paged_attention()]
+                     for k, *rest in getattr(self.model.blocks[c.layer].mixer, "paged_attention", tuple)()]
             self._beam_layers = sorted(set(found))
         native = self.native is not None and not recorded and self.debug_hook is None and not KernelProfiler.enabled
         n, seen = len(lens), []

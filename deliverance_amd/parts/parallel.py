@@ -39,7 +39,7 @@ class ParallelMixer(Mixer):
         return tuple(b.cache_need() for b in self.branches)
 
     def paged_attention(self):
-        return tuple((k, *rest) for k, b in enumerate(self.branches) for _, *rest in b.paged_attention())
+        return tuple((k, *rest) for k, b in enumerate(self.branches) for _, *rest in getattr(b, "paged_attention", tuple)())
 
     def forward(self, ctx: StepContext, h: torch.Tensor, x: torch.Tensor, call) -> None:
         accumulate = ctx.part_accumulate

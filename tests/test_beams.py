@@ -454,6 +454,9 @@ def test_what_a_step_of_beams_is_judged_by(beams_library, monkeypatch):
     attend = StepRunner._beams_attend(runner, BeamStep(2, 4, [0.0] * 4, [[0, 0], [16, 16]]), [70, 110], 4, 16, recorded=False)
     assert asked == [((95, 0), 46.0), ((63, 0), 46.0)] and attend == frozenset()
     assert StepRunner._beams_attend(runner, BeamStep(1, 4, [0.0] * 2, [[64, 64], [64, 64]]), [70, 70], 2, 16, recorded=True) == frozenset()
+    runner.model.blocks[:] = [N(mixer=N()), layers[1]]        # (a mixer of a user's own that says nothing of its attention)
+    runner._beam_layers, runner._beam_choices = None, {}
+    assert StepRunner._beams_attend(runner, step, [70, 110], 8, 16, recorded=True) == {(1, 4, 2, 64, 50)}
 
 
 def test_the_estimate_of_unusual_steps(beams_library):
